@@ -8,6 +8,8 @@ fails loudly if the shared library has not been built - there is no fallback.
 """
 from __future__ import annotations
 
+import collections
+import contextlib
 import ctypes
 import os
 
@@ -166,6 +168,39 @@ class rt_gemm_params_t(ctypes.Structure):
                                                "flags")]
 
 
+class rt_kv8_append_params_t(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_uint32) for n in ("num_seqs", "num_kv_heads", "num_tokens",
+                                               "max_pages_per_seq")] + [
+        (n, ctypes.c_uint64) for n in ("arena_pages", "k_stride", "v_stride")] + [
+        ("format", ctypes.c_uint32), ("dtype", ctypes.c_uint32)]
+
+
+class rt_kv8_attn_params_t(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_uint32) for n in ("num_seqs", "num_q_heads", "num_kv_heads",
+                                               "max_pages_per_seq", "max_seq_len", "format")] + [
+        ("arena_pages", ctypes.c_uint64), ("q_stride", ctypes.c_uint64),
+        ("scale", ctypes.c_float), ("chunk_pages", ctypes.c_uint32)]
+
+
+class rt_logprob_params_t(ctypes.Structure):
+    _fields_ = [("num_rows", ctypes.c_uint32), ("vocab", ctypes.c_uint32),
+                ("row_stride", ctypes.c_uint64), ("grad_stride", ctypes.c_uint64),
+                ("dtype", ctypes.c_uint32), ("temperature", ctypes.c_float),
+                ("row_enable", ctypes.c_void_p)]
+
+
+class rt_policy_params_t(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_uint32) for n in ("num_rows", "vocab", "num_seqs", "dtype")] + [
+        ("row_stride", ctypes.c_uint64), ("grad_stride", ctypes.c_uint64)] + [
+        (n, ctypes.c_float) for n in ("temperature", "clip_low", "clip_high", "kl_coef",
+                                      "entropy_coef")]
+
+
+class rt_policy_row_t(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_float) for n in ("logprob", "entropy", "loss", "policy", "kl",
+                                              "ratio", "clipped", "weight")]
+
+
 class rt_decode_worker_stats_t(ctypes.Structure):
     _fields_ = [("consumed", ctypes.c_uint64), ("completed", ctypes.c_uint64)] + [
         (n, ctypes.c_uint32) for n in ("published", "sentinels", "comp_ring_full")] + [
@@ -210,6 +245,14 @@ _SIGS = {
                                                          ctypes.POINTER(rt_attn_group_params_t)]
                                           + [_P] * 9 + [ctypes.c_size_t, _P]),
     "rt_attn_workspace_error": (ctypes.c_int, [_P, _P, ctypes.POINTER(ctypes.c_int32)]),
+    "rt_kv8_append": (ctypes.c_int, [ctypes.POINTER(rt_kv8_append_params_t)] + [_P] * 10),
+    "rt_kv8_attn_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(rt_kv8_attn_params_t)]),
+    "rt_kv8_decode_attention": (ctypes.c_int, [ctypes.POINTER(rt_kv8_attn_params_t)] + [_P] * 8
+                                + [ctypes.c_size_t, _P, _P]),
+    "rt_token_logprobs": (ctypes.c_int, [ctypes.POINTER(rt_logprob_params_t)] + [_P] * 6),
+    "rt_token_logprobs_backward": (ctypes.c_int, [ctypes.POINTER(rt_logprob_params_t)]
+                                   + [_P] * 7),
+    "rt_policy_loss": (ctypes.c_int, [ctypes.POINTER(rt_policy_params_t)] + [_P] * 12),
     "rt_sample_rows": (ctypes.c_int, [ctypes.POINTER(rt_sample_params_t), _P, _P, _P, _P]),
     "rt_sample_uniform24": (ctypes.c_uint32, [ctypes.c_uint64, ctypes.c_uint32, ctypes.c_uint64]),
     "rt_chunk_max_stride": (ctypes.c_uint32, [ctypes.c_uint32]),
@@ -414,6 +457,148 @@ class GroupedDecodeAttention(PagedDecodeAttention):
             _ptr(out), _ptr(self.workspace), self.workspace.numel(), _stream_ptr(stream)),
             "rt_paged_decode_attention_grouped")
         return out
+
+
+# -------------------------------------------------------------- 8-bit cache
+RT_DTYPE_F32, RT_DTYPE_BF16 = 0, 1
+RT_KV8_E4M3, RT_KV8_S8 = 0, 1
+KV8_PLANE_BYTES = 2048
+
+
+def _need(ok, what):
+    if not ok:
+        raise ValueError(what)
+
+
+def _same_device(first, *others):
+    """Every tensor given lies on the first one's CUDA device."""
+    dev = first.device
+    _need(dev.type == "cuda", "tensors must be on a CUDA device")
+    for t in others:
+        _need(t is None or t.device == dev, "tensors must be on one device")
+    return dev
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(dev, stream):
+    """A context in which the tensors' device is current, and `stream` where one is given (so
+    that what is allocated inside belongs to the stream that uses it), and the stream's handle."""
+    import torch
+    if stream is not None:
+        _need(stream.device == dev, "the stream is another device's")
+        return torch.cuda.stream(stream), stream.cuda_stream
+    s = torch.cuda.current_stream(dev).cuda_stream
+    return (_HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)), s
+
+
+def _error_word(error):
+    import torch
+    if error is None:
+        return None
+    _need(error.dtype == torch.int32 and error.numel() == 1, "error: one int32")
+    return error.data_ptr()
+
+
+def _int_array(t, shape, what):
+    import torch
+    _need(t.dtype == torch.int32 and t.shape == shape and t.is_contiguous(),
+          f"{what}: contiguous int32 {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+def _kv8_cache(pages, scales, tail, num_seqs):
+    """(format, KV heads) of a cache's buffers, checked."""
+    import torch
+    fmt = {torch.float8_e4m3fn: RT_KV8_E4M3, torch.int8: RT_KV8_S8}.get(pages.dtype)
+    _need(fmt is not None, f"pages: float8_e4m3fn or int8, got {pages.dtype}")
+    _need(pages.dim() == 4 and tuple(pages.shape[2:]) == (2, KV8_PLANE_BYTES)
+          and pages.is_contiguous(), "pages: contiguous [n, kv heads, 2, 2048]")
+    n, h = pages.shape[:2]
+    _need(scales.dtype == torch.float32 and scales.shape == (n, h, 2) and scales.is_contiguous(),
+          "scales: contiguous float32 [n, kv heads, 2]")
+    _need(tail.dtype == torch.bfloat16 and tail.shape == (num_seqs, h, 2, 16, 128)
+          and tail.is_contiguous(), "tail: contiguous bfloat16 [sequences, kv heads, 2, 16, 128]")
+    return fmt, h
+
+
+def kv8_cache(n_pages, num_seqs, num_kv_heads, format="e4m3", device="cuda"):
+    """Empty buffers (pages, scales, tail) of an 8-bit KV cache; format "e4m3" or "s8"."""
+    import torch
+    _need(format in ("e4m3", "s8"), f"format: 'e4m3' or 's8', got {format!r}")
+    pages = torch.zeros(n_pages, num_kv_heads, 2, KV8_PLANE_BYTES, dtype=torch.int8, device=device)
+    if format == "e4m3":
+        pages = pages.view(torch.float8_e4m3fn)
+    return (pages, torch.zeros(n_pages, num_kv_heads, 2, device=device),
+            torch.zeros(num_seqs, num_kv_heads, 2, 16, 128, dtype=torch.bfloat16, device=device))
+
+
+def kv8_append(k, v, cu_tokens, seq_lens, page_table, pages, scales, tail, error=None,
+               stream=None):
+    """rt_kv8_append: tokens cu_tokens[b] .. cu_tokens[b + 1] of k and v (bf16 or fp32
+    [T, kv heads, 128], any token stride that is a multiple of 8) behind the seq_lens[b]
+    tokens that sequence b has.  cu_tokens int32 [B + 1], seq_lens int32 [B], page_table
+    int32 [B, P]; pages, scales and tail as kv8_cache makes them.  seq_lens is not advanced."""
+    import torch
+    B = seq_lens.shape[0]
+    dev = _same_device(pages, k, v, cu_tokens, seq_lens, page_table, scales, tail, error)
+    fmt, h = _kv8_cache(pages, scales, tail, B)
+    dtype = {torch.float32: RT_DTYPE_F32, torch.bfloat16: RT_DTYPE_BF16}.get(k.dtype)
+    _need(dtype is not None and v.dtype == k.dtype, "k, v: both bfloat16 or both float32")
+    T = k.shape[0]
+    for t in (k, v):
+        _need(t.shape == (T, h, 128) and t.stride(2) == 1 and (h == 1 or t.stride(1) == 128),
+              "k, v: [tokens, kv heads, 128] with contiguous heads")
+    _need(page_table.dim() == 2 and page_table.shape[0] == B, "page_table: int32 [sequences, P]")
+    strides = [t.stride(0) if T > 1 else h * 128 for t in (k, v)]
+    p = rt_kv8_append_params_t(B, h, T, page_table.shape[1], pages.shape[0], *strides, fmt, dtype)
+    args = (_int_array(cu_tokens, (B + 1,), "cu_tokens"), _int_array(seq_lens, (B,), "seq_lens"),
+            _int_array(page_table, page_table.shape, "page_table"))
+    ctx, s = _on(dev, stream)
+    with ctx:
+        check(lib().rt_kv8_append(ctypes.byref(p), k.data_ptr(), v.data_ptr(), *args,
+                                  pages.data_ptr(), scales.data_ptr(), tail.data_ptr(),
+                                  _error_word(error), s), "rt_kv8_append")
+
+
+def kv8_decode_attention(q, pages, scales, tail, page_table, seq_lens, max_seq_len, scale=None,
+                         out=None, chunk_pages=0, workspace=None, error=None, stream=None):
+    """rt_kv8_decode_attention: q bf16 [B, Hq, 128] over the cache of kv8_append; returns
+    fp32 [B, Hq, 128].  max_seq_len bounds every seq_lens[b].  workspace: uint8, by default
+    a new one (from torch's allocator, on the current stream)."""
+    import torch
+    B = seq_lens.shape[0]
+    dev = _same_device(q, pages, scales, tail, page_table, seq_lens, out, workspace, error)
+    fmt, h = _kv8_cache(pages, scales, tail, B)
+    _need(q.dtype == torch.bfloat16 and q.dim() == 3 and q.shape[0] == B and q.shape[2] == 128
+          and q.stride(2) == 1 and (q.shape[1] == 1 or q.stride(1) == 128),
+          "q: bfloat16 [sequences, heads, 128] with contiguous heads")
+    Hq = q.shape[1]
+    _need(out is None or (out.dtype == torch.float32 and out.shape == (B, Hq, 128)
+                          and out.is_contiguous()),
+          "out: contiguous float32 [sequences, heads, 128]")
+    _need(page_table.dim() == 2 and page_table.shape[0] == B, "page_table: int32 [sequences, P]")
+    _need(0 <= max_seq_len <= 0x7FFFFFFF and 0 <= chunk_pages <= 128,
+          "max_seq_len 0 .. 2^31 - 1, chunk_pages 0 .. 128")
+    p = rt_kv8_attn_params_t(B, Hq, h, page_table.shape[1], max_seq_len, fmt, pages.shape[0],
+                             q.stride(0) if B > 1 else Hq * 128,
+                             scale if scale is not None else 128 ** -0.5, chunk_pages)
+    args = (_int_array(page_table, page_table.shape, "page_table"),
+            _int_array(seq_lens, (B,), "seq_lens"))
+    ctx, s = _on(dev, stream)
+    with ctx:
+        if out is None:
+            out = torch.empty(B, Hq, 128, dtype=torch.float32, device=dev)
+        need = lib().rt_kv8_attn_workspace_bytes(ctypes.byref(p))
+        if need and workspace is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        check(lib().rt_kv8_decode_attention(
+            ctypes.byref(p), q.data_ptr(), pages.data_ptr(), scales.data_ptr(), tail.data_ptr(),
+            *args, out.data_ptr(), None if workspace is None else workspace.data_ptr(),
+            0 if workspace is None else workspace.numel() * workspace.element_size(),
+            _error_word(error), s), "rt_kv8_decode_attention")
+    return out
 
 
 def fill_normal_bf16(t, seed, stream_id=0, mean=0.0, std=1.0, stream=None):
@@ -889,6 +1074,129 @@ def grpo_advantages(rewards, group, eps=1e-6, out=None, stream=None):
     check(lib().rt_grpo_advantages(_ptr(rewards), rewards.numel(), group, eps, _ptr(out),
                                    _stream_ptr(stream)), "rt_grpo_advantages")
     return out
+
+
+def _rows_of(logits, tokens):
+    """(rows, vocab, row stride, dtype) of a matrix of logits and its tokens, checked."""
+    import torch
+    dtype = {torch.float32: RT_DTYPE_F32, torch.bfloat16: RT_DTYPE_BF16}.get(logits.dtype)
+    _need(dtype is not None and logits.dim() == 2, "logits: bfloat16 or float32 [rows, vocab]")
+    R, V = logits.shape
+    _need(V == 1 or logits.stride(1) == 1, "logits: contiguous rows")
+    _need(tokens.dtype in (torch.int32, torch.uint32) and tokens.shape == (R,)
+          and tokens.is_contiguous(), "tokens: contiguous int32 [rows]")
+    return R, V, (logits.stride(0) if R > 1 else V), dtype
+
+
+def _float_array(t, n, what):
+    import torch
+    if t is None:
+        return None
+    _need(t.dtype == torch.float32 and t.shape == (n,) and t.is_contiguous(),
+          f"{what}: contiguous float32 [{n}], got {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+def _index_array(t, n, what):
+    import torch
+    if t is None:
+        return None
+    _need(t.dtype in (torch.int32, torch.uint32) and t.shape == (n,) and t.is_contiguous(),
+          f"{what}: contiguous int32 [{n}]")
+    return t.data_ptr()
+
+
+def _gradient_of(logits, dlogits):
+    """The gradient's buffer (a new one for None) and its row stride."""
+    import torch
+    R, V = logits.shape
+    if dlogits is None:
+        dlogits = torch.empty(R, V, dtype=logits.dtype, device=logits.device)
+    _need(dlogits.dtype == logits.dtype and dlogits.shape == logits.shape
+          and (V == 1 or dlogits.stride(1) == 1), "dlogits: the logits' type and shape")
+    return dlogits, (dlogits.stride(0) if R > 1 else V)
+
+
+def token_logprobs(logits, tokens, temperature=1.0, row_enable=None, logprobs=None, entropy=None,
+                   error=None, stream=None):
+    """rt_token_logprobs: (log-probability of each row's token, entropy of each row), fp32 [R],
+    of logits fp32 or bf16 [R, V] (any row stride) and tokens int32 [R].  Rows whose row_enable
+    (int32 [R]) is 0 are skipped: give logprobs and entropy to know what they hold."""
+    import torch
+    R, V, stride, dtype = _rows_of(logits, tokens)
+    dev = _same_device(logits, tokens, row_enable, logprobs, entropy, error)
+    p = rt_logprob_params_t(R, V, stride, 0, dtype, temperature,
+                            _index_array(row_enable, R, "row_enable"))
+    ctx, s = _on(dev, stream)
+    with ctx:
+        if logprobs is None:
+            logprobs = torch.empty(R, dtype=torch.float32, device=dev)
+        if entropy is None:
+            entropy = torch.empty(R, dtype=torch.float32, device=dev)
+        check(lib().rt_token_logprobs(ctypes.byref(p), logits.data_ptr(), tokens.data_ptr(),
+                                      _float_array(logprobs, R, "logprobs"),
+                                      _float_array(entropy, R, "entropy"), _error_word(error), s),
+              "rt_token_logprobs")
+    return logprobs, entropy
+
+
+def token_logprobs_backward(logits, tokens, dlogprobs, dentropy=None, temperature=1.0,
+                            row_enable=None, dlogits=None, error=None, stream=None):
+    """rt_token_logprobs_backward: the gradient with respect to the logits, in their type;
+    dlogits may be the logits themselves."""
+    R, V, stride, dtype = _rows_of(logits, tokens)
+    dev = _same_device(logits, tokens, dlogprobs, dentropy, row_enable, dlogits, error)
+    ctx, s = _on(dev, stream)
+    with ctx:
+        dlogits, grad_stride = _gradient_of(logits, dlogits)
+        p = rt_logprob_params_t(R, V, stride, grad_stride, dtype, temperature,
+                                _index_array(row_enable, R, "row_enable"))
+        check(lib().rt_token_logprobs_backward(
+            ctypes.byref(p), logits.data_ptr(), tokens.data_ptr(),
+            _float_array(dlogprobs, R, "dlogprobs"), _float_array(dentropy, R, "dentropy"),
+            dlogits.data_ptr(), _error_word(error), s), "rt_token_logprobs_backward")
+    return dlogits
+
+
+# stats fp32 [5]: weighted sums of loss, policy, kl, entropy, clipped; then fp32 [R] columns of
+# the rows' records (rt_policy_row_t) and the gradient (None when not asked for)
+PolicyLoss = collections.namedtuple(
+    "PolicyLoss", "stats logprobs entropy row_loss policy kl ratio clipped dlogits")
+
+
+def policy_loss(logits, tokens, weights, advantages, old_logprobs=None, ref_logprobs=None,
+                row_seq=None, *, temperature=1.0, clip_low=0.2, clip_high=0.2, kl_coef=0.0,
+                entropy_coef=0.0, backward=True, dlogits=None, error=None, stream=None):
+    """rt_policy_loss: the clipped policy loss of rows of logits (fp32 or bf16 [R, V]) and its
+    gradient.  weights fp32 [R]; advantages fp32 [S], one per rollout, with row_seq int32 [R]
+    naming each row's (None: one per row); old_logprobs None: on-policy.  dlogits may be the
+    logits themselves; backward=False computes the values alone.  Returns a PolicyLoss."""
+    import torch
+    R, V, stride, dtype = _rows_of(logits, tokens)
+    dev = _same_device(logits, tokens, weights, advantages, old_logprobs, ref_logprobs, row_seq,
+                       dlogits, error)
+    _need(backward or dlogits is None, "dlogits without backward")
+    _need(advantages.dim() == 1 and (row_seq is not None or advantages.shape[0] == R),
+          "advantages: one per row without row_seq")
+    ctx, s = _on(dev, stream)
+    with ctx:
+        grad_stride = 0
+        if backward:
+            dlogits, grad_stride = _gradient_of(logits, dlogits)
+        rows = torch.empty(R, 8, dtype=torch.float32, device=dev)
+        stats = torch.empty(5, dtype=torch.float32, device=dev)
+        p = rt_policy_params_t(R, V, advantages.shape[0], dtype, stride, grad_stride, temperature,
+                               clip_low, clip_high, kl_coef, entropy_coef)
+        check(lib().rt_policy_loss(
+            ctypes.byref(p), logits.data_ptr(), tokens.data_ptr(),
+            _float_array(weights, R, "weights"),
+            _float_array(advantages, advantages.shape[0], "advantages"),
+            _index_array(row_seq, R, "row_seq"), _float_array(old_logprobs, R, "old_logprobs"),
+            _float_array(ref_logprobs, R, "ref_logprobs"), rows.data_ptr(), stats.data_ptr(),
+            None if dlogits is None else dlogits.data_ptr(), _error_word(error), s),
+            "rt_policy_loss")
+    c = rows.unbind(1)
+    return PolicyLoss(stats, c[0], c[1], c[2], c[3], c[4], c[5], c[6], dlogits)
 
 
 class NcclRewards:

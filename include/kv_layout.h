@@ -108,3 +108,42 @@ rt_page_bytes(uint32_t num_kv_heads)
 {
     return (uint64_t)num_kv_heads * 2u * RT_PAGE_TOKENS * RT_HEAD_DIM * 2u;
 }
+
+/* ---- 8-bit paged GQA layout -------------------------------------------
+ * One page holds RT_PAGE_TOKENS tokens of one sequence for every KV head, one
+ * byte an element; plane 0 is K, plane 1 is V:
+ *
+ *     byte  ((p * Hkv + h) * 2 + plane) * 2048 + rt_kv8_{k,v}_offset(t, d)
+ *     scale fp32 [p][h][plane];  value = scale * code
+ *
+ * so each (page, head) is 4 KiB of contiguous codes (one bulk copy).  Inside a
+ * plane the bytes lie in the order in which a warp feeds them to m16n8k16
+ * tensor-core products: 16-byte vector j * 32 + lane is what `lane` holds of
+ * quarter j, with four tokens' (V) or four dimensions' (K) bytes to a word.
+ * Only full pages exist in this form; the tokens of a sequence's unfinished
+ * page stay in bf16, in that sequence's entry of a "tail" buffer with the
+ * bf16 page layout above (page index = sequence index). */
+#define RT_KV8_PLANE_BYTES 2048u
+
+/* Byte of (token t, dimension d) inside a K plane. */
+static inline RT_HD uint32_t
+rt_kv8_k_offset(uint32_t t, uint32_t d)
+{
+    return (d / 32u) * 512u + ((t % 8u) * 4u + (d / 4u) % 4u) * 16u +
+           (2u * ((d / 16u) % 2u) + t / 8u) * 4u + d % 4u;
+}
+
+/* Byte of (token t, dimension d) inside a V plane. */
+static inline RT_HD uint32_t
+rt_kv8_v_offset(uint32_t t, uint32_t d)
+{
+    return (d / 32u) * 512u + ((d % 8u) * 4u + (t % 8u) / 2u) * 16u +
+           (2u * ((d / 16u) % 2u) + (d / 8u) % 2u) * 4u + t % 2u + 2u * (t / 8u);
+}
+
+/* Bytes of one 8-bit page for all KV heads (scales apart). */
+static inline RT_HD uint64_t
+rt_kv8_page_bytes(uint32_t num_kv_heads)
+{
+    return (uint64_t)num_kv_heads * 2u * RT_KV8_PLANE_BYTES;
+}

@@ -173,6 +173,90 @@ int rt_attn_plan(const rt_attn_params_t *p, uint32_t *chunk_pages,
                  uint32_t *max_chunks, uint64_t *ctas);
 
 /* ------------------------------------------------------------------------
+ * KV cache in 8 bits (no reference counterpart): half the HBM traffic of the
+ * bf16 pages, which bounds decode attention.
+ *
+ * Every (page, KV head, plane) tile x of 16 tokens x 128 dimensions has one
+ * fp32 scale, and every element one code:
+ *     scale = max|x| / Q          (Q = 448 for e4m3, 127 for s8; one fp32 division)
+ *     code  = round(x / scale)    (fp32 quotient, then to nearest even; |code| <= Q)
+ * with scale = 0 and codes 0 for a tile of zeros, and scale = NaN when a tile
+ * holds a NaN or an infinity (attention over it is then NaN, as over the
+ * values themselves).  Tiles are quantised once, when their 16 tokens are
+ * there: a sequence of L tokens has L / 16 pages in 8 bits (page_table) and
+ * its last L % 16 tokens in bf16, in its entry of `tail`.  So the cache does
+ * not depend on how many tokens each call brought, and full pages, which are
+ * never written again, can be shared by sequences with a common prefix.
+ *
+ *   pages  codes, [arena_pages] pages of rt_kv8_page_bytes, order of kv_layout.h
+ *   scales fp32 [arena_pages][num_kv_heads][2] (K, V)
+ *   tail   bf16 [num_seqs] pages in the bf16 page layout of kv_layout.h
+ *
+ * `error` is a device int32 (or NULL: not reported) that a call sets, when it
+ * is 0, to the code of a bad index it met and skipped: 1 = a length that is
+ * negative or beyond max_pages_per_seq (attention: or max_seq_len), 2 = a page
+ * id outside the arena, 3 = cu_tokens decreases or leaves [0, num_tokens],
+ * 4 = a bounded wait expired (never expected).  Pointers are 16-byte aligned
+ * unless said otherwise.
+ * ---------------------------------------------------------------------- */
+#define RT_DTYPE_F32  0u
+#define RT_DTYPE_BF16 1u
+#define RT_KV8_E4M3   0u
+#define RT_KV8_S8     1u
+
+typedef struct {
+    uint32_t num_seqs;
+    uint32_t num_kv_heads;
+    uint32_t num_tokens;         /* rows of k and v */
+    uint32_t max_pages_per_seq;  /* page-table row stride */
+    uint64_t arena_pages;
+    uint64_t k_stride, v_stride; /* elements between tokens, >= num_kv_heads * 128 and a
+                                    multiple of 8 (so k and v may be columns of one
+                                    projection's output) */
+    uint32_t format;             /* RT_KV8_* */
+    uint32_t dtype;              /* RT_DTYPE_* of k and v */
+} rt_kv8_append_params_t;
+
+/* Append tokens [cu_tokens[b], cu_tokens[b + 1]) of k and v (each row
+ * [num_kv_heads][128]) to sequence b, which holds seq_lens[b] tokens; any
+ * count, 0 included, for each b (int32 device arrays, 4-byte aligned).  fp32
+ * rows are rounded to bf16 first.  Pages that become full are quantised to
+ * page_table[b][position / 16]; the tokens of the unfinished page go to
+ * tail[b], whose other rows stay as they were.  The lengths are the caller's
+ * to advance afterwards.  Page ids written by one call must differ. */
+int rt_kv8_append(const rt_kv8_append_params_t *p, const void *k, const void *v,
+                  const int32_t *cu_tokens, const int32_t *seq_lens, const int32_t *page_table,
+                  void *pages, float *scales, void *tail, int32_t *error, void *stream);
+
+typedef struct {
+    uint32_t num_seqs;
+    uint32_t num_q_heads;        /* a multiple of num_kv_heads, 1 to 8 to a KV head */
+    uint32_t num_kv_heads;
+    uint32_t max_pages_per_seq;  /* page-table row stride */
+    uint32_t max_seq_len;        /* upper bound on every seq_lens[b] */
+    uint32_t format;             /* RT_KV8_* */
+    uint64_t arena_pages;
+    uint64_t q_stride;           /* elements between sequences' queries, >= num_q_heads * 128
+                                    and a multiple of 8 */
+    float    scale;              /* softmax scale, usually 1/sqrt(128) */
+    uint32_t chunk_pages;        /* pages per work item, up to 128; 0 = auto */
+} rt_kv8_attn_params_t;
+
+/* Decode attention over the 8-bit cache: rt_paged_decode_attention with
+ * K = scale * code.  q bf16 [num_seqs][num_q_heads][128] (rows q_stride
+ * apart), out fp32 [num_seqs][num_q_heads][128]; a sequence of length 0 gives
+ * zeros, one skipped for an error is left as it was.  `workspace` holds the
+ * partial results of sequences that are split (0 bytes when max_seq_len fits
+ * one item); it needs no initialisation, and calls that share one must not
+ * overlap on the GPU.  Results do not depend on earlier calls and are the
+ * same, bit for bit, in every run of a shape. */
+size_t rt_kv8_attn_workspace_bytes(const rt_kv8_attn_params_t *p);
+int rt_kv8_decode_attention(const rt_kv8_attn_params_t *p, const void *q, const void *pages,
+                            const float *scales, const void *tail, const int32_t *page_table,
+                            const int32_t *seq_lens, float *out, void *workspace,
+                            size_t workspace_bytes, int32_t *error, void *stream);
+
+/* ------------------------------------------------------------------------
  * Fused sampler (replaces reference cu/sample.cu:40-123 sample_token).
  *
  * One call samples one token per row of fp32 logits with the reference's
@@ -666,6 +750,83 @@ int rt_kv_branch_resolve(const KVPrefixTable *table, const uint32_t *branch_ids,
  * correctly rounded, no fused multiply-add).  n must be a multiple of G. */
 int rt_grpo_advantages(const float *rewards, uint32_t n, uint32_t G, float eps, float *adv,
                        void *stream);
+
+/* ------------------------------------------------------------------------
+ * Log-probabilities and the policy loss: the step of a GRPO update behind
+ * rt_grpo_advantages (no reference counterpart).
+ *
+ * Row r has logits l[r][0 .. vocab) (fp32 or bf16) and one token t.  With
+ * z = l / temperature (temperature 0: z = l, as the sampler), p = softmax(z):
+ *     lp = z[t] - log(sum exp z)          H = -sum p log p
+ *     d lp / d l[v] = ([v = t] - p[v]) / temperature
+ *     d H  / d l[v] = -p[v] (log p[v] + H) / temperature
+ * A logit of -infinity has p = 0 and gradient 0; a row that holds a NaN or
+ * +infinity, or nothing but -infinity, gives NaN.  Sums are kept in fp32 or
+ * more; a gradient is rounded once, to the logits' type.
+ *
+ * Rows are row_stride elements apart (any value >= vocab), and start at any
+ * multiple of their element's size; a gradient may be written over its logits
+ * (the same address and stride), else the memory from the first row's start to
+ * the last row's end must not overlap.  `error` is a device int32 (or NULL)
+ * set, when it is 0, to 1 for a token >= vocab and 2 for a row_seq >= num_seqs
+ * (4 = a bounded wait expired, never expected); such a row's outputs and
+ * gradient are 0, as those of a row of weight 0.
+ * ---------------------------------------------------------------------- */
+typedef struct {
+    uint32_t num_rows;
+    uint32_t vocab;              /* 1 .. 262144 */
+    uint64_t row_stride;         /* elements between rows of logits */
+    uint64_t grad_stride;        /* elements between rows of dlogits */
+    uint32_t dtype;              /* RT_DTYPE_* of logits and dlogits */
+    float    temperature;        /* 0, or 1e-4 .. 1e4 */
+    const uint32_t *row_enable;  /* device [num_rows] or NULL: rows whose flag is 0 are not
+                                    read; forward leaves their outputs untouched, backward
+                                    gives them a gradient of 0 */
+} rt_logprob_params_t;
+
+/* logprobs and entropy fp32 [num_rows] (entropy may be NULL). */
+int rt_token_logprobs(const rt_logprob_params_t *p, const void *logits, const uint32_t *tokens,
+                      float *logprobs, float *entropy, int32_t *error, void *stream);
+
+/* dlogits = dlogprobs d lp + dentropy d H (fp32 [num_rows]; dentropy may be
+ * NULL: 0).  Recomputes the softmax: each logit is read once. */
+int rt_token_logprobs_backward(const rt_logprob_params_t *p, const void *logits,
+                               const uint32_t *tokens, const float *dlogprobs,
+                               const float *dentropy, void *dlogits, int32_t *error,
+                               void *stream);
+
+/* Clipped policy loss.  Row r belongs to the rollout s = row_seq[r] (NULL: s = r)
+ * with advantage A = advantages[s]:
+ *     ratio  = exp(lp - old_logprobs[r])   (old_logprobs NULL: on-policy, ratio 1)
+ *     policy = -min(ratio A, clip(ratio, 1 - clip_low, 1 + clip_high) A)
+ *     kl     = exp(ref - lp) - (ref - lp) - 1      (ref_logprobs; when kl_coef != 0)
+ *     loss   = policy + kl_coef kl - entropy_coef H
+ * and the call's loss is sum_r weights[r] loss_r.  The clipped branch has no
+ * gradient; it is taken where ratio A exceeds the clipped product.  A row of
+ * weight 0 (padding) is not read; its record and its gradient are 0. */
+typedef struct {
+    uint32_t num_rows;
+    uint32_t vocab;              /* 1 .. 262144 */
+    uint32_t num_seqs;           /* entries of advantages (row_seq NULL: >= num_rows) */
+    uint32_t dtype;
+    uint64_t row_stride, grad_stride;
+    float    temperature;
+    float    clip_low, clip_high;   /* >= 0 */
+    float    kl_coef, entropy_coef; /* finite */
+} rt_policy_params_t;
+
+typedef struct {                 /* one per row, 16-byte aligned */
+    float logprob, entropy, loss, policy;
+    float kl, ratio, clipped, weight;
+} rt_policy_row_t;
+
+/* rows [num_rows]; stats fp32 [5] = sum over rows of weight x {loss, policy,
+ * kl, entropy, clipped}, added in fp64 in a fixed order; dlogits = d (sum of
+ * weight x loss) / d logits, or NULL for the forward values alone. */
+int rt_policy_loss(const rt_policy_params_t *p, const void *logits, const uint32_t *tokens,
+                   const float *weights, const float *advantages, const uint32_t *row_seq,
+                   const float *old_logprobs, const float *ref_logprobs, rt_policy_row_t *rows,
+                   float *stats, void *dlogits, int32_t *error, void *stream);
 
 /* NCCL plumbing for the one cross-GPU exchange of the path: every rank
  * contributes its rollouts' rewards, every rank receives all of them in
