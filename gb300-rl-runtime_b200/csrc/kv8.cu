@@ -194,16 +194,16 @@ __global__ void __launch_bounds__(kAppendWarps * 32) kv8_append_kernel(const App
 
 // --------------------------------------------------------------- attention
 constexpr int kWarps = 4;
-constexpr int kStages = 4;
+constexpr int kStages = 2;
 constexpr int kCtasPerSm = 3;
-constexpr uint32_t kBlockBytes = 2 * kPlane;              // one (page, head): K plane, V plane
-constexpr uint32_t kRingBytes = kWarps * kStages * kBlockBytes;
-constexpr uint32_t kTailBytes = 2 * 16 * 256;             // bf16 K and V rows of the tail
-constexpr uint32_t kHeadPitch = 132;                      // floats per head of the warps' merge
-constexpr int kSmemBytes = kRingBytes + kTailBytes;
-constexpr uint32_t kMaxChunkPages = 32 * kWarps;          // one page id per lane
+constexpr uint32_t kBlockBytes = 2 * kPlane;       // one (page, head): K plane, V plane
+constexpr uint32_t kEntryBytes = 2 * kBlockBytes;  // two pages, or a tail's K and V rows
+constexpr uint32_t kHeadPitch = 132;               // floats per column of the warps' merge
+constexpr int kSmemBytes = kWarps * kStages * kEntryBytes;
+constexpr uint32_t kMaxChunkPages = 32 * kWarps;   // a page to a lane
+constexpr int kMergeWarps = 16;
 constexpr uint64_t kWaitLimitNs = 2000000000ull;
-static_assert(kWarps * 8 * kHeadPitch * 4 <= kRingBytes, "the merge reuses the ring");
+static_assert(kWarps * 8 * kHeadPitch * 4 <= kSmemBytes, "the merge reuses the ring");
 
 struct AttnArgs {
     const __nv_bfloat16 *q;
@@ -241,14 +241,42 @@ __device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// The same for 32 codes a row: the cache's own format against the query's digits.
+template <uint32_t FMT>
+__device__ __forceinline__ void mma_codes_16832(uint32_t (&d)[4], const uint4 &a, uint32_t b0,
+                                                uint32_t b1)
+{
+    if constexpr (FMT == RT_KV8_E4M3)
+        asm volatile(
+            "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 "
+            "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+            : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+    else
+        asm volatile(
+            "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 "
+            "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+            : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+template <uint32_t FMT>
+__device__ __forceinline__ float sum_of(uint32_t d)
+{
+    return FMT == RT_KV8_E4M3 ? __uint_as_float(d) : (float)(int32_t)d;
+}
+
 // Four codes as two fp16 pairs, exactly.  s8: with its sign bit flipped a
 // code c is the byte c + 128, and 0x6400 | byte is the fp16 1024 + byte.
 template <uint32_t FMT>
 __device__ __forceinline__ void decode4(uint32_t w, uint32_t &lo, uint32_t &hi)
 {
     if constexpr (FMT == RT_KV8_E4M3) {
-        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(lo) : "h"((uint16_t)(w & 0xFFFFu)));
-        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(hi) : "h"((uint16_t)(w >> 16)));
+        asm("{\n\t.reg .b16 a, b;\n\t"
+            "mov.b32 {a, b}, %2;\n\t"
+            "cvt.rn.f16x2.e4m3x2 %0, a;\n\t"
+            "cvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+            : "=r"(lo), "=r"(hi)
+            : "r"(w));
     } else {
         const uint32_t u = w ^ 0x80808080u;
         const __half2 bias = __half2half2(__ushort_as_half(0x6480));  // 1152
@@ -272,18 +300,44 @@ __device__ __forceinline__ float2 unpack_f16x2(uint32_t v)
 }
 
 // State of one warp's online softmax over its tokens, base 2: lane (g, c) =
-// (lane / 4, lane % 4) has the heads 2c and 2c + 1, and of O^T the dimensions
+// (lane / 4, lane % 4) has the columns 2c and 2c + 1, and of O^T the dimensions
 // 16 i + g (o[i][0], o[i][1]) and 16 i + 8 + g (o[i][2], o[i][3]).
 struct Softmax {
     float m0, m1, l0, l1;
     float o[8][4];
+    int v;  // O's unit is 2^(v - 14), the same in all lanes
 };
 
-// New maxima for scores of 16 tokens (rows g and g + 8); s becomes exp2(s - m).
-// Returns the factors for what was summed before.
-__device__ __forceinline__ float2 softmax_step(Softmax &st, float (&s)[4])
+__device__ __forceinline__ float exp2i(int e) { return __int_as_float((127 + e) << 23); }
+
+// Bring O to a unit that holds V scales of up to `top` (bits of a float, no sign).
+__device__ __forceinline__ void raise_unit(Softmax &st, uint32_t top)
 {
-    float x0 = fmaxf(s[0], s[2]), x1 = fmaxf(s[1], s[3]);
+    const int v = min((int)(top >> 23) - 126, 127);
+    if (v > st.v) {
+        // from -110 the step can be 237: in two factors
+        const float f = exp2i(max(st.v - v, -126)), f2 = exp2i(min(0, st.v - v + 126));
+        st.v = v;
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+                st.o[i][u] = st.o[i][u] * f * f2;
+    }
+}
+
+// New maxima for the scores of NP times 16 tokens (rows g and g + 8); s becomes
+// exp2(s - m), and what was summed before is brought to the new maxima.  A warp
+// in which no maximum has moved leaves O alone (the factor is exactly 1).
+template <int NP>
+__device__ __forceinline__ void softmax_step(Softmax &st, float (&s)[NP][4])
+{
+    float x0 = fmaxf(s[0][0], s[0][2]), x1 = fmaxf(s[0][1], s[0][3]);
+#pragma unroll
+    for (int p = 1; p < NP; p++) {
+        x0 = fmaxf(x0, fmaxf(s[p][0], s[p][2]));
+        x1 = fmaxf(x1, fmaxf(s[p][1], s[p][3]));
+    }
 #pragma unroll
     for (int off = 4; off < 32; off <<= 1) {
         x0 = fmaxf(x0, __shfl_xor_sync(0xFFFFFFFFu, x0, off));
@@ -291,39 +345,376 @@ __device__ __forceinline__ float2 softmax_step(Softmax &st, float (&s)[4])
     }
     x0 = fmaxf(x0, st.m0);
     x1 = fmaxf(x1, st.m1);
-    const float2 f = make_float2(rt::fast_exp2(st.m0 - x0), rt::fast_exp2(st.m1 - x1));
-    st.m0 = x0;
-    st.m1 = x1;
-    s[0] = rt::fast_exp2(s[0] - x0);
-    s[2] = rt::fast_exp2(s[2] - x0);
-    s[1] = rt::fast_exp2(s[1] - x1);
-    s[3] = rt::fast_exp2(s[3] - x1);
-    st.l0 = st.l0 * f.x + (s[0] + s[2]);
-    st.l1 = st.l1 * f.y + (s[1] + s[3]);
-    return f;
+    if (__any_sync(0xFFFFFFFFu, x0 != st.m0 || x1 != st.m1)) {
+        const float f0 = rt::fast_exp2(st.m0 - x0), f1 = rt::fast_exp2(st.m1 - x1);
+        st.m0 = x0;
+        st.m1 = x1;
+        st.l0 *= f0;
+        st.l1 *= f1;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            st.o[i][0] *= f0;
+            st.o[i][1] *= f1;
+            st.o[i][2] *= f0;
+            st.o[i][3] *= f1;
+        }
+    }
+#pragma unroll
+    for (int p = 0; p < NP; p++) {
+        s[p][0] = rt::fast_exp2(s[p][0] - x0);
+        s[p][2] = rt::fast_exp2(s[p][2] - x0);
+        s[p][1] = rt::fast_exp2(s[p][1] - x1);
+        s[p][3] = rt::fast_exp2(s[p][3] - x1);
+        st.l0 += s[p][0] + s[p][2];
+        st.l1 += s[p][1] + s[p][3];
+    }
 }
 
-// One CTA per (sequence, KV head, chunk of pages), its warps taking the pages
-// in turn.  A page's K and V codes are one 4 KiB bulk copy into the warp's
-// ring.  Math per page: S^T = K.Q^T and O^T = V^T.P^T on m16n8k16 with the 16
-// tokens (or 16 dimensions) as rows and the KV group's heads as columns.  Codes
-// are exact in fp16; a query row is scaled by a power of two into fp16's range
-// (exact for all that matters in fp32: see load_q) and the scales of K and V
-// are applied in fp32, to the scores and to the page's part of O.  P is split
-// into two fp16 terms, which keeps 22 bits of it.
-template <uint32_t FMT>
+// The query in the codes' own format.  With an element q scaled by a power of
+// two, s8 writes the integer nearest to it in digits of base 256, each in [-128,
+// 127]; e4m3 writes it as a sum of terms t_i 2^-4i, each the nearest to 16 times
+// what the ones before have left.  Products with codes are exact and their sums
+// kept in fp32 or integers, so K needs no conversion: a word of it is an operand
+// as it lies.
+//
+// Up to 4 heads to a KV head (DUP): 4 digits, the 8 columns of one product taking
+// two of them (columns 0..3 the one, 4..7 the other) and a second product the
+// other two.  More heads: 3 digits in 3 products.  What is lost of an element is
+// below 2^-30 (2^-22 with 3 digits of s8, 2^-26 with 3 of e4m3) of the row's
+// largest.  bf16's 8 bits fill two terms of e4m3 unless an element is below 2^-13
+// of the largest, so most rows need no more (`deep` is false).
+template <uint32_t FMT, bool DUP>
+struct Query {
+    static constexpr int kDigits = DUP ? 4 : 3, kProducts = DUP ? 2 : 3;
+    uint32_t f[kProducts][4][2];
+    float k0, k1;  // factors of the scores of the lane's columns 2c and 2c + 1
+    bool deep;     // e4m3: digits past the second are not all 0 (the same in all lanes)
+
+    // Lane (g, c) holds, of column g, dimensions 16 s + 4 c .. + 3 for s = 0..7, as
+    // K's words hold them.
+    __device__ __forceinline__ void load(const __nv_bfloat16 *row, bool has, float scale_log2)
+    {
+        const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+        uint2 qv[8];
+#pragma unroll
+        for (int s = 0; s < 8; s++)
+            qv[s] = has ? *reinterpret_cast<const uint2 *>(row + 16 * s + 4 * c) : make_uint2(0u, 0u);
+        uint32_t top2 = 0;
+#pragma unroll
+        for (int s = 0; s < 8; s++)
+            top2 = __vmaxu2(top2, __vmaxu2(qv[s].x & 0x7FFF7FFFu, qv[s].y & 0x7FFF7FFFu));
+        uint32_t top = max(top2 & 0xFFFFu, top2 >> 16);
+        top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+        top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+        // The row times 2^(kTop - e), its largest element in [2^kTop, 2^(kTop + 1)): a
+        // first digit of up to 127 (s8, with room for the carry) or 256 (e4m3).
+        constexpr int kTop = FMT == RT_KV8_E4M3 ? 7 : 8 * kDigits - 3;
+        const int e = min(max((int)(top >> 7) - 127, kTop - 126), 127);
+        const float up = exp2i(kTop - e);
+        // a row with a NaN or an infinity has no digits: its scores become NaN
+        const float down = top >= 0x7F80u ? __int_as_float(0x7FC00000) : exp2i(e - kTop);
+        auto element = [&](int s, int u) {
+            const uint32_t w = u & 2 ? qv[s].y : qv[s].x;
+            return __uint_as_float(u & 1 ? w & 0xFFFF0000u : w << 16) * up;
+        };
+        deep = true;
+        if constexpr (FMT == RT_KV8_E4M3) {
+            // the first term cut off after 4 bits, the second has the other 4
+            bool small = false;
+#pragma unroll
+            for (int s = 0; s < 8; s++) {
+                uint32_t t0 = 0, t1 = 0;
+#pragma unroll
+                for (int u = 0; u < 4; u += 2) {
+                    const float x = element(s, u), y = element(s, u + 1);
+                    const float xh = __uint_as_float(__float_as_uint(x) & 0xFFF00000u);
+                    const float yh = __uint_as_float(__float_as_uint(y) & 0xFFF00000u);
+                    // below 2^-6 a term is not exact
+                    small |= (fabsf(x) < 0.015625f && x != 0.0f) || (fabsf(y) < 0.015625f && y != 0.0f);
+                    t0 |= term(xh, yh) << (8 * u);
+                    t1 |= term((x - xh) * 16.0f, (y - yh) * 16.0f) << (8 * u);
+                }
+                if constexpr (DUP) {
+                    f[0][s >> 1][s & 1] = g < 4 ? t0 : t1;
+                    f[1][s >> 1][s & 1] = 0u;
+                } else {
+                    f[0][s >> 1][s & 1] = t0;
+                    f[1][s >> 1][s & 1] = t1;
+                    f[2][s >> 1][s & 1] = 0u;
+                }
+            }
+            deep = __any_sync(0xFFFFFFFFu, small);
+            if (deep) {
+#pragma unroll 1
+                for (int half = 0; half < 2; half++) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        uint32_t d[kDigits];
+#pragma unroll
+                        for (int i = 0; i < kDigits; i++)
+                            d[i] = 0;
+#pragma unroll
+                        for (int u = 0; u < 4; u += 2) {
+                            float x = half ? element(2 * j + 1, u) : element(2 * j, u);
+                            float y = half ? element(2 * j + 1, u + 1) : element(2 * j, u + 1);
+#pragma unroll
+                            for (int i = 0; i < kDigits; i++) {
+                                const uint32_t t = term(x, y);
+                                uint32_t back;
+                                asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(back) : "h"((uint16_t)t));
+                                const float2 v = unpack_f16x2(back);
+                                x = (x - v.x) * 16.0f;
+                                y = (y - v.y) * 16.0f;
+                                d[i] |= t << (8 * u);
+                            }
+                        }
+#pragma unroll
+                        for (int i = 0; i < kProducts; i++) {
+                            const uint32_t w = DUP ? (g < 4 ? d[2 * i] : d[(2 * i + 1) % kDigits]) : d[i];
+                            if (half)
+                                f[i][j][1] = w;
+                            else
+                                f[i][j][0] = w;
+                        }
+                    }
+                }
+            }
+        } else {
+            // A byte plus 128, carried on, less 128 is a digit: all of them at once.
+            constexpr uint32_t kBias = DUP ? 0x00808080u : 0x00008080u;
+            // bytes of the first and second product's digits, as selectors
+            const uint32_t s0 = DUP ? (g < 4 ? 0x73u : 0x62u) : 0x62u;
+            const uint32_t s1 = DUP ? (g < 4 ? 0x51u : 0x40u) : 0x51u;
+#pragma unroll
+            for (int s = 0; s < 8; s++) {
+                uint32_t n[4];
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+                    n[u] = ((uint32_t)__float2int_rn(element(s, u)) + kBias) ^ kBias;
+                auto digit = [&](uint32_t sel) {
+                    return __byte_perm(__byte_perm(n[0], n[1], sel), __byte_perm(n[2], n[3], sel), 0x5410);
+                };
+                f[0][s >> 1][s & 1] = digit(s0);
+                f[1][s >> 1][s & 1] = digit(s1);
+                if constexpr (!DUP)
+                    f[2][s >> 1][s & 1] = digit(0x40u);
+            }
+        }
+        k0 = scale_log2 * __shfl_sync(0xFFFFFFFFu, down, 8 * c);
+        k1 = scale_log2 * __shfl_sync(0xFFFFFFFFu, down, 8 * c + 4);
+    }
+
+    static __device__ __forceinline__ uint32_t term(float x, float y)
+    {
+        uint16_t t;
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(t) : "f"(y), "f"(x));
+        return t;
+    }
+
+    // Scores of the 16 tokens of a K plane, but for K's scale: x[0], x[1] columns 2c,
+    // 2c + 1 of token g, x[2], x[3] of token g + 8.
+    __device__ __forceinline__ void scores(const uint4 *k, float (&x)[4]) const
+    {
+        uint32_t d[kProducts][4];
+#pragma unroll
+        for (int i = 0; i < kProducts; i++)
+            d[i][0] = d[i][1] = d[i][2] = d[i][3] = 0u;
+        constexpr int kFirst = FMT == RT_KV8_S8 ? kProducts : DUP ? 1 : 2;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const uint4 w = k[j * 32];
+#pragma unroll
+            for (int i = 0; i < kFirst; i++)
+                mma_codes_16832<FMT>(d[i], w, f[i][j][0], f[i][j][1]);
+        }
+        if (kFirst < kProducts && deep) {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                mma_codes_16832<FMT>(d[kProducts - 1], k[j * 32], f[kProducts - 1][j][0],
+                                     f[kProducts - 1][j][1]);
+        }
+        constexpr float kBase = FMT == RT_KV8_E4M3 ? 0.0625f : 256.0f;
+        if constexpr (DUP) {
+            // digits 0 and 2 in columns 0..3, 1 and 3 in 4..7
+            const bool low = (threadIdx.x & 2) != 0;
+            const float one = FMT == RT_KV8_E4M3 ? (low ? kBase : 1.0f)
+                                                 : (low ? kBase * kBase : kBase * kBase * kBase);
+            const float two = FMT == RT_KV8_E4M3 ? one * kBase * kBase : (low ? 1.0f : kBase);
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                x[u] = fmaf(sum_of<FMT>(d[0][u]), one, sum_of<FMT>(d[1][u]) * two);
+                x[u] += __shfl_xor_sync(0xFFFFFFFFu, x[u], 2);
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const float a = sum_of<FMT>(d[0][u]), b = sum_of<FMT>(d[1][u]), c = sum_of<FMT>(d[2][u]);
+                x[u] = FMT == RT_KV8_E4M3 ? fmaf(fmaf(c, kBase, b), kBase, a)
+                                          : fmaf(fmaf(a, kBase, b), kBase, c);
+            }
+        }
+    }
+};
+
+// NP pages of codes with the scales sk of K and sv of V: scores, softmax, and
+// P.V added to O.
+template <uint32_t FMT, bool DUP, int NP>
+__device__ __forceinline__ void pages_step(Softmax &st, const uint4 *(&blk)[NP],
+                                           const Query<FMT, DUP> &q, const float (&sk)[NP],
+                                           const float (&sv)[NP])
+{
+    float x[NP][4];
+#pragma unroll
+    for (int p = 0; p < NP; p++) {
+        q.scores(blk[p], x[p]);
+        const float f0 = sk[p] * q.k0, f1 = sk[p] * q.k1;
+        x[p][0] *= f0;
+        x[p][1] *= f1;
+        x[p][2] *= f0;
+        x[p][3] *= f1;
+    }
+    softmax_step<NP>(st, x);
+    uint32_t top = __float_as_uint(sv[0]) & 0x7FFFFFFFu;
+    if constexpr (NP > 1)
+        top = max(top, __float_as_uint(sv[1]) & 0x7FFFFFFFu);
+    raise_unit(st, top);
+    const bool low_half = DUP && (threadIdx.x & 2) != 0;  // columns 4..7
+#pragma unroll
+    for (int p = 0; p < NP; p++) {
+        const float vf = sv[p] * exp2i(14 - st.v);
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+            x[p][u] *= vf;
+        // P as two fp16 terms, transposed into the second product's B operand
+        const uint32_t h0 = pack_f16x2(x[p][0], x[p][1]), h1 = pack_f16x2(x[p][2], x[p][3]);
+        const float2 r0 = unpack_f16x2(h0), r1 = unpack_f16x2(h1);
+        const uint32_t l0 = pack_f16x2(x[p][0] - r0.x, x[p][1] - r0.y);
+        const uint32_t l1 = pack_f16x2(x[p][2] - r1.x, x[p][3] - r1.y);
+        const uint32_t p0 = rt::movmatrix_trans(low_half ? l0 : h0);
+        const uint32_t p1 = rt::movmatrix_trans(low_half ? l1 : h1);
+        uint32_t q0 = 0, q1 = 0;
+        if constexpr (!DUP) {
+            q0 = rt::movmatrix_trans(l0);
+            q1 = rt::movmatrix_trans(l1);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const uint4 w = blk[p][128 + j * 32];
+            uint32_t f[4];
+            decode4<FMT>(w.x, f[0], f[2]);
+            decode4<FMT>(w.y, f[1], f[3]);
+            mma_f16_16816(st.o[2 * j], f, p0, p1);
+            if constexpr (!DUP)
+                mma_f16_16816(st.o[2 * j], f, q0, q1);
+            decode4<FMT>(w.z, f[0], f[2]);
+            decode4<FMT>(w.w, f[1], f[3]);
+            mma_f16_16816(st.o[2 * j + 1], f, p0, p1);
+            if constexpr (!DUP)
+                mma_f16_16816(st.o[2 * j + 1], f, q0, q1);
+        }
+    }
+}
+
+// The bf16 tail, n_tail tokens of [16][128] K and V rows in shared memory: the
+// same products on bf16 fragments, P in three bf16 terms (24 bits).  Rows past
+// the tail's end hold anything: their scores are -inf and their V bits cleared.
+// With DUP the first four columns carry all three terms.
+template <bool DUP>
+__device__ __forceinline__ void tail_step(Softmax &st, const uint8_t *tk, const uint8_t *tv,
+                                          const __nv_bfloat16 *q_row, bool has_q, uint32_t n_tail,
+                                          float scale_log2)
+{
+    const int g = (threadIdx.x & 31) >> 2, c = threadIdx.x & 3;
+    float x[1][4] = {{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+    for (int s = 0; s < 8; s++) {
+        const uint2 qv = has_q ? *reinterpret_cast<const uint2 *>(q_row + 16 * s + 4 * c)
+                               : make_uint2(0u, 0u);
+        const uint2 a0 = *reinterpret_cast<const uint2 *>(tk + g * 256 + (16 * s + 4 * c) * 2);
+        const uint2 a1 = *reinterpret_cast<const uint2 *>(tk + (g + 8) * 256 + (16 * s + 4 * c) * 2);
+        const uint32_t f[4] = {a0.x, a1.x, a0.y, a1.y};
+        rt::mma_bf16_16816(x[0], f, qv.x, qv.y);
+    }
+    const bool in0 = (uint32_t)g < n_tail, in1 = (uint32_t)g + 8u < n_tail;
+    x[0][0] = in0 ? x[0][0] * scale_log2 : -INFINITY;
+    x[0][1] = in0 ? x[0][1] * scale_log2 : -INFINITY;
+    x[0][2] = in1 ? x[0][2] * scale_log2 : -INFINITY;
+    x[0][3] = in1 ? x[0][3] * scale_log2 : -INFINITY;
+    softmax_step<1>(st, x);
+    uint32_t p[3][2];
+    raise_unit(st, 0x3F800000u);
+    const float unit = DUP && (threadIdx.x & 2) ? 0.0f : exp2i(14 - st.v);
+#pragma unroll
+    for (int u = 0; u < 4; u++)
+        x[0][u] *= unit;
+#pragma unroll
+    for (int k = 0; k < 3; k++) {
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const uint32_t w = rt::pack_bf16x2(x[0][2 * u], x[0][2 * u + 1]);
+            x[0][2 * u] -= __uint_as_float(w << 16);
+            x[0][2 * u + 1] -= __uint_as_float(w & 0xFFFF0000u);
+            p[k][u] = rt::movmatrix_trans(w);
+        }
+    }
+    // lane c's tokens: 2c, 2c + 1 and 2c + 8, 2c + 9
+    auto keep = [&](uint32_t t) {
+        return (t < n_tail ? 0xFFFFu : 0u) | (t + 1u < n_tail ? 0xFFFF0000u : 0u);
+    };
+    const uint32_t keep0 = keep(2 * c), keep1 = keep(2 * c + 8);
+    const uint16_t *v16 = reinterpret_cast<const uint16_t *>(tv);
+    auto pair = [&](uint32_t t, uint32_t d) {
+        return (uint32_t)v16[t * 128 + d] | (uint32_t)v16[(t + 1) * 128 + d] << 16;
+    };
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const uint32_t d0 = 16 * i + g;
+        const uint32_t f[4] = {pair(2 * c, d0) & keep0, pair(2 * c, d0 + 8) & keep0,
+                               pair(2 * c + 8, d0) & keep1, pair(2 * c + 8, d0 + 8) & keep1};
+#pragma unroll
+        for (int k = 0; k < 3; k++)
+            rt::mma_bf16_16816(st.o[i], f, p[k][0], p[k][1]);
+    }
+}
+
+// One CTA per (sequence, KV head, chunk of pages), the pairs of pages dealt out to
+// its warps.  Each warp has a ring of entries that bulk copies fill: the K and V
+// codes of two pages for the KV head, or the tail's K and V rows.  The CTAs are
+// handed out by the hardware, chunk by chunk of the whole batch: warps differ by
+// 10% in the bandwidth they get, and equal shares dealt out beforehand end when
+// the slowest does.
+//
+// Math, two pages at a time: S^T = K.Q^T with the codes as they are and the query
+// in digits (Query), O^T += V^T.P^T on m16n8k16 with the codes in fp16, exactly;
+// 16 tokens (or 16 dimensions) as rows, the KV group's heads as columns.  K's
+// scale multiplies the scores in fp32.  V's multiplies P: with O's unit 2^(v -
+// 14), v the exponent above the largest scale so far, P times scale fills fp16's
+// range from 2^14 down to 2^-24, and two fp16 terms of it are off by 2^-38 of the
+// largest scale or 2^-22 of their own value.  With up to 4 heads (DUP) columns
+// 4..7 repeat columns 0..3 and carry P's low terms, so one product covers both.
+template <uint32_t FMT, bool DUP>
 __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) kv8_decode_kernel(const AttnArgs a)
 {
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ __align__(8) uint64_t bars[kWarps][kStages];
-    __shared__ __align__(8) uint64_t tail_bar;
     __shared__ float2 ml[kWarps][8];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int g = lane >> 2, c = lane & 3;
-    const uint32_t h = blockIdx.x % a.num_kv_heads;
-    const uint32_t rest = blockIdx.x / a.num_kv_heads;
+    const uint32_t H = a.num_kv_heads, G = a.G;
+    rt::grid_dep_launch();
+    const uint32_t h = blockIdx.x % H, rest = blockIdx.x / H;
     const uint32_t b = rest % a.num_seqs, chunk = rest / a.num_seqs;
+    const uint32_t p0 = chunk * a.chunk_pages;
+    // Lane l has page l & 1 of the warp's pair l / 2: pair warp + kWarps (l / 2) of the
+    // chunk.  Its id is read beside the length, which then says whether it counts.
+    const uint32_t my_page = p0 + 2u * ((uint32_t)warp + kWarps * ((uint32_t)lane >> 1)) + (lane & 1);
+    const bool in_table = my_page < a.max_pages && my_page < p0 + a.chunk_pages;
     const int32_t L = a.lens[b];
+    const int32_t id = in_table ? a.page_table[(uint64_t)b * a.max_pages + my_page] : -1;
+    const uint32_t head = DUP ? (uint32_t)g & 3u : (uint32_t)g;
+    const bool has_q = head < G;
+    const __nv_bfloat16 *q_row = a.q + (uint64_t)b * a.q_stride + ((uint64_t)h * G + head) * 128u;
+
     if (!len_ok(a, L)) {
         if (threadIdx.x == 0 && chunk == 0)
             flag_error(a.error, kErrLen);
@@ -332,331 +723,278 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) kv8_decode_kernel(con
     const uint32_t n_chunks = chunks_of(a, L);
     if (chunk >= n_chunks)
         return;
-    const uint32_t G = a.G;
-    const uint32_t n_full = (uint32_t)L >> 4;
-    const uint32_t p0 = chunk * a.chunk_pages;
-    const uint32_t p1 = min(n_full, p0 + a.chunk_pages);
-    const uint32_t n_tail = chunk + 1 == n_chunks ? (uint32_t)L & 15u : 0u;
-    int n_mine = (int)((p1 - p0 + kWarps - 1 - warp) / kWarps);
+    const uint32_t p1 = min((uint32_t)L >> 4, p0 + a.chunk_pages);
+    const uint32_t pairs = (p1 - p0 + 1u) / 2u;
+    const uint32_t n_pairs = (pairs + kWarps - 1u - (uint32_t)warp) / kWarps;
+    // the tail goes to the first warp with the fewest pairs
+    const uint32_t n_tail =
+        chunk + 1 == n_chunks && (uint32_t)warp == pairs % kWarps ? (uint32_t)L & 15u : 0u;
+    const uint32_t n_entries = n_pairs + (n_tail ? 1u : 0u);
 
-    // barriers: each warp its own; warp 0 the tail's
     if (lane == 0) {
 #pragma unroll
         for (int s = 0; s < kStages; s++)
             rt::mbar_init(rt::smem_u32(&bars[warp][s]), 1);
-        if (warp == 0)
-            rt::mbar_init(rt::smem_u32(&tail_bar), 1);
         rt::mbar_fence_init();
     }
     __syncwarp();
+    const bool mine = in_table && my_page < p1, ok = mine && id >= 0 && (uint64_t)id < a.arena_pages;
+    if (mine && !ok)
+        flag_error(a.error, kErrPage);
+    const uint32_t have = __ballot_sync(0xFFFFFFFFu, ok);  // pages that are read
+    const uint64_t block = ok ? (uint64_t)id * H + h : 0u;
+    const uint32_t ring = rt::smem_u32(smem) + (uint32_t)warp * kStages * kEntryBytes;
 
-    // this warp's page ids and scales, one page per lane; -1: not read
-    int32_t id = -1;
-    float2 sc = make_float2(0.0f, 0.0f);
-    if (lane < n_mine) {
-        id = a.page_table[(size_t)b * a.max_pages + p0 + warp + lane * kWarps];
-        if (id < 0 || (uint64_t)id >= a.arena_pages) {
-            flag_error(a.error, kErrPage);
-            id = -1;
-        } else {
-            sc = *reinterpret_cast<const float2 *>(a.scales +
-                                                   ((uint64_t)id * a.num_kv_heads + h) * 2u);
+    uint32_t issued = 0;
+    auto issue = [&]() {
+        const uint32_t s = issued % kStages;
+        const uint32_t bar = rt::smem_u32(&bars[warp][s]), dst = ring + s * kEntryBytes;
+        if (issued < n_pairs) {
+            if ((uint32_t)lane >> 1 == issued) {
+                const uint32_t both = have >> (2u * issued) & 3u, odd = lane & 1;
+                if (!odd && both)
+                    rt::mbar_arrive_expect_tx(bar, both == 3u ? 2u * kBlockBytes : kBlockBytes);
+                if (ok)
+                    rt::bulk_load(dst + odd * kBlockBytes, a.pages + block * kBlockBytes, kBlockBytes, bar);
+            }
+        } else if (lane == 0) {
+            const __nv_bfloat16 *t = a.tail + rt_page_elem_offset(b, h, 0, 0, H);
+            rt::mbar_arrive_expect_tx(bar, n_tail * 512u);
+            rt::bulk_load(dst, t, n_tail * 256u, bar);
+            rt::bulk_load(dst + kBlockBytes, t + 2048, n_tail * 256u, bar);
         }
-    }
-    const uint32_t ring = rt::smem_u32(smem) + (uint32_t)warp * kStages * kBlockBytes;
-    auto issue = [&](int i) {
-        const int32_t pg = __shfl_sync(0xFFFFFFFFu, id, i);
-        if (lane == 0 && pg >= 0) {
-            const uint32_t s = (uint32_t)i % kStages;
-            const uint32_t bar = rt::smem_u32(&bars[warp][s]);
-            rt::mbar_arrive_expect_tx(bar, kBlockBytes);
-            rt::bulk_load(ring + s * kBlockBytes,
-                          a.pages + ((uint64_t)pg * a.num_kv_heads + h) * kBlockBytes, kBlockBytes,
-                          bar);
-        }
+        issued++;
     };
-    for (int i = 0; i < kStages && i < n_mine; i++)
-        issue(i);
-    const uint32_t tail_s = rt::smem_u32(smem) + kRingBytes;
-    const int tail_warp = (int)((p1 - p0) % kWarps);  // the first one with fewer pages
-    if (n_tail && warp == 0 && lane == 0) {
-        const uint32_t bar = rt::smem_u32(&tail_bar), bytes = n_tail * 256u;
-        const __nv_bfloat16 *src = a.tail + rt_page_elem_offset(b, h, 0, 0, a.num_kv_heads);
-        rt::mbar_arrive_expect_tx(bar, 2 * bytes);
-        rt::bulk_load(tail_s, src, bytes, bar);
-        rt::bulk_load(tail_s + 4096u, src + 2048, bytes, bar);
-    }
+    while (issued < (uint32_t)kStages && issued < n_entries)
+        issue();
+    const float2 sc = ok ? *reinterpret_cast<const float2 *>(a.scales + block * 2u) : make_float2(0.f, 0.f);
 
-    // Query fragments: lane (g, c) holds, of head g, dimensions 16 s + 4 c .. + 3
-    // for step s, as K's words hold them.  The row is multiplied by a power of
-    // two so that its largest element lies in [2^14, 2^15): bf16 elements down to
-    // 2^-31 of that are exact in fp16, and what the smaller ones lose is below
-    // 2^-39 of the largest.
-    const __nv_bfloat16 *q_row = a.q + (uint64_t)b * a.q_stride + ((uint64_t)h * G + g) * 128u;
-    uint2 qv[8];
-#pragma unroll
-    for (int s = 0; s < 8; s++)
-        qv[s] = (uint32_t)g < G ? *reinterpret_cast<const uint2 *>(q_row + 16 * s + 4 * c)
-                                : make_uint2(0u, 0u);
-    uint32_t top2 = 0;
-#pragma unroll
-    for (int s = 0; s < 8; s++)
-        top2 = __vmaxu2(top2, __vmaxu2(qv[s].x & 0x7FFF7FFFu, qv[s].y & 0x7FFF7FFFu));
-    uint32_t top = max(top2 & 0xFFFFu, top2 >> 16);
-    top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-    top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-    // 2^(14 - e) for a largest element of exponent e; within fp32's normal range
-    const int e = min(max((int)(top >> 7) - 127, -112), 126);
-    const float up = __int_as_float((127 + 14 - e) << 23), down = __int_as_float((127 - 14 + e) << 23);
-    uint32_t qf[8][2];
-#pragma unroll
-    for (int s = 0; s < 8; s++) {
-        qf[s][0] = pack_f16x2(__uint_as_float(qv[s].x << 16) * up,
-                              __uint_as_float(qv[s].x & 0xFFFF0000u) * up);
-        qf[s][1] = pack_f16x2(__uint_as_float(qv[s].y << 16) * up,
-                              __uint_as_float(qv[s].y & 0xFFFF0000u) * up);
-    }
-    const float k0 = a.scale_log2 * __shfl_sync(0xFFFFFFFFu, down, 8 * c);       // head 2c
-    const float k1 = a.scale_log2 * __shfl_sync(0xFFFFFFFFu, down, 8 * c + 4);   // head 2c + 1
-
+    Query<FMT, DUP> q;
+    q.load(q_row, has_q, a.scale_log2);
     Softmax st;
     st.m0 = st.m1 = -INFINITY;
     st.l0 = st.l1 = 0.0f;
+    st.v = -110;
 #pragma unroll
     for (int i = 0; i < 8; i++)
         st.o[i][0] = st.o[i][1] = st.o[i][2] = st.o[i][3] = 0.0f;
 
-    int n_issue = n_mine;
-    uint32_t phases = 0;
-    for (int i = 0; i < n_mine; i++) {
-        const int32_t pg = __shfl_sync(0xFFFFFFFFu, id, i);
-        const float sk = __shfl_sync(0xFFFFFFFFu, sc.x, i), sv = __shfl_sync(0xFFFFFFFFu, sc.y, i);
-        const uint32_t s = (uint32_t)i % kStages;
-        if (pg >= 0) {
-            // after an expired wait no page is issued any more; those in flight are
-            // waited for, each again with a limit
-            if (!__all_sync(0xFFFFFFFFu,
-                            rt::mbar_wait_bounded(rt::smem_u32(&bars[warp][s]), (phases >> s) & 1u,
-                                                  kWaitLimitNs))) {
+    const uint8_t *slots = smem + (uint32_t)warp * kStages * kEntryBytes;
+    uint32_t phases = 0, limit = n_entries;
+    for (uint32_t i = 0; i < issued; i++) {
+        const uint32_t s = i % kStages;
+        const uint32_t both = i < n_pairs ? have >> (2u * i) & 3u : 4u;
+        if (both) {
+            // After an expired wait nothing is issued any more; what is in flight is
+            // waited for, each entry again with a limit.
+            if (!__all_sync(0xFFFFFFFFu, rt::mbar_wait_bounded(rt::smem_u32(&bars[warp][s]),
+                                                               (phases >> s) & 1u, kWaitLimitNs))) {
                 if (lane == 0)
                     flag_error(a.error, kErrTimeout);
-                n_issue = 0;
-                n_mine = min(n_mine, i + kStages);
+                limit = 0;
             }
             phases ^= 1u << s;
-            const uint4 *blk = reinterpret_cast<const uint4 *>(smem + (ring - rt::smem_u32(smem)) +
-                                                               s * kBlockBytes) + lane;
-            float sa[4] = {0.f, 0.f, 0.f, 0.f}, sb[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const uint4 w = blk[j * 32];
-                uint32_t f[4];
-                decode4<FMT>(w.x, f[0], f[2]);
-                decode4<FMT>(w.y, f[1], f[3]);
-                mma_f16_16816(sa, f, qf[2 * j][0], qf[2 * j][1]);
-                decode4<FMT>(w.z, f[0], f[2]);
-                decode4<FMT>(w.w, f[1], f[3]);
-                mma_f16_16816(sb, f, qf[2 * j + 1][0], qf[2 * j + 1][1]);
+            const uint8_t *base = slots + s * kEntryBytes;
+            const uint4 *blk0 = reinterpret_cast<const uint4 *>(base) + lane;
+            const uint4 *blk1 = blk0 + kBlockBytes / 16;
+            if (both == 3u) {
+                const uint4 *blk[2] = {blk0, blk1};
+                const float sk[2] = {__shfl_sync(0xFFFFFFFFu, sc.x, 2 * i),
+                                     __shfl_sync(0xFFFFFFFFu, sc.x, 2 * i + 1)};
+                const float sv[2] = {__shfl_sync(0xFFFFFFFFu, sc.y, 2 * i),
+                                     __shfl_sync(0xFFFFFFFFu, sc.y, 2 * i + 1)};
+                pages_step<FMT, DUP, 2>(st, blk, q, sk, sv);
+            } else if (both == 4u) {
+                tail_step<DUP>(st, base, base + kBlockBytes, q_row, has_q, n_tail, a.scale_log2);
+            } else {
+                const uint4 *blk[1] = {both == 1u ? blk0 : blk1};
+                const int k = 2 * i + (both == 1u ? 0 : 1);
+                const float sk[1] = {__shfl_sync(0xFFFFFFFFu, sc.x, k)};
+                const float sv[1] = {__shfl_sync(0xFFFFFFFFu, sc.y, k)};
+                pages_step<FMT, DUP, 1>(st, blk, q, sk, sv);
             }
-            const float f0 = sk * k0, f1 = sk * k1;
-            float x[4] = {(sa[0] + sb[0]) * f0, (sa[1] + sb[1]) * f1, (sa[2] + sb[2]) * f0,
-                          (sa[3] + sb[3]) * f1};
-            const float2 fac = softmax_step(st, x);
-            // P as two fp16 terms, transposed into the second product's B operand
-            const uint32_t h0 = pack_f16x2(x[0], x[1]), h1 = pack_f16x2(x[2], x[3]);
-            const float2 r0 = unpack_f16x2(h0), r1 = unpack_f16x2(h1);
-            const uint32_t l0 = pack_f16x2(x[0] - r0.x, x[1] - r0.y);
-            const uint32_t l1 = pack_f16x2(x[2] - r1.x, x[3] - r1.y);
-            const uint32_t ph0 = rt::movmatrix_trans(h0), ph1 = rt::movmatrix_trans(h1);
-            const uint32_t pl0 = rt::movmatrix_trans(l0), pl1 = rt::movmatrix_trans(l1);
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const uint4 w = blk[128 + j * 32];
-                uint32_t f[4];
-                float d[4] = {0.f, 0.f, 0.f, 0.f}, d2[4] = {0.f, 0.f, 0.f, 0.f};
-                decode4<FMT>(w.x, f[0], f[2]);
-                decode4<FMT>(w.y, f[1], f[3]);
-                mma_f16_16816(d, f, ph0, ph1);
-                mma_f16_16816(d, f, pl0, pl1);
-                decode4<FMT>(w.z, f[0], f[2]);
-                decode4<FMT>(w.w, f[1], f[3]);
-                mma_f16_16816(d2, f, ph0, ph1);
-                mma_f16_16816(d2, f, pl0, pl1);
-#pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    const float fu = u & 1 ? fac.y : fac.x;
-                    st.o[2 * j][u] = fmaf(d[u], sv, st.o[2 * j][u] * fu);
-                    st.o[2 * j + 1][u] = fmaf(d2[u], sv, st.o[2 * j + 1][u] * fu);
-                }
-            }
+            __syncwarp();  // every lane has read the slot before it is filled again
         }
-        __syncwarp();  // every lane has read the slot before it is filled again
-        if (i + kStages < n_issue)
-            issue(i + kStages);
+        if (issued < limit)
+            issue();
     }
 
-    // The bf16 tail: the same products on bf16 fragments, P in three bf16 terms.
-    // Rows past the tail's end hold anything: their scores are -inf and their V
-    // bits are cleared.
-    __syncthreads();  // tail_bar is initialised
-    if (n_tail && warp == tail_warp) {
-        if (!rt::mbar_wait_bounded(rt::smem_u32(&tail_bar), 0, kWaitLimitNs))
-            flag_error(a.error, kErrTimeout);
-        const uint8_t *tk = smem + kRingBytes, *tv = tk + 4096;
-        float x[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int s = 0; s < 8; s++) {
-            const uint2 a0 = *reinterpret_cast<const uint2 *>(tk + g * 256 + (16 * s + 4 * c) * 2);
-            const uint2 a1 = *reinterpret_cast<const uint2 *>(tk + (g + 8) * 256 + (16 * s + 4 * c) * 2);
-            const uint32_t f[4] = {a0.x, a1.x, a0.y, a1.y};
-            rt::mma_bf16_16816(x, f, qv[s].x, qv[s].y);
-        }
-        const bool in0 = (uint32_t)g < n_tail, in1 = (uint32_t)g + 8u < n_tail;
-        x[0] = in0 ? x[0] * a.scale_log2 : -INFINITY;
-        x[1] = in0 ? x[1] * a.scale_log2 : -INFINITY;
-        x[2] = in1 ? x[2] * a.scale_log2 : -INFINITY;
-        x[3] = in1 ? x[3] * a.scale_log2 : -INFINITY;
-        const float2 fac = softmax_step(st, x);
-        uint32_t p[3][2];
-#pragma unroll
-        for (int k = 0; k < 3; k++) {
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const uint32_t w = rt::pack_bf16x2(x[2 * u], x[2 * u + 1]);
-                x[2 * u] -= __uint_as_float(w << 16);
-                x[2 * u + 1] -= __uint_as_float(w & 0xFFFF0000u);
-                p[k][u] = rt::movmatrix_trans(w);
-            }
-        }
-        // lane c's tokens: 2c, 2c + 1 and 2c + 8, 2c + 9
-        auto keep = [&](uint32_t t) {
-            return (t < n_tail ? 0xFFFFu : 0u) | (t + 1u < n_tail ? 0xFFFF0000u : 0u);
-        };
-        const uint32_t keep0 = keep(2 * c), keep1 = keep(2 * c + 8);
-        const uint16_t *v16 = reinterpret_cast<const uint16_t *>(tv);
-        auto pair = [&](uint32_t t, uint32_t d) {
-            return (uint32_t)v16[t * 128 + d] | (uint32_t)v16[(t + 1) * 128 + d] << 16;
-        };
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const uint32_t d0 = 16 * i + g;
-            const uint32_t f[4] = {pair(2 * c, d0) & keep0, pair(2 * c, d0 + 8) & keep0,
-                                   pair(2 * c + 8, d0) & keep1, pair(2 * c + 8, d0 + 8) & keep1};
-#pragma unroll
-            for (int u = 0; u < 4; u++)
-                st.o[i][u] *= u & 1 ? fac.y : fac.x;
-#pragma unroll
-            for (int k = 0; k < 3; k++)
-                rt::mma_bf16_16816(st.o[i], f, p[k][0], p[k][1]);
-        }
-    }
-
-    // Merge the warps: sums over a head's lanes, then all states through shared memory.
+    // Merge the warps: sums over a column's lanes, then all states through shared memory.
 #pragma unroll
     for (int off = 4; off < 32; off <<= 1) {
         st.l0 += __shfl_xor_sync(0xFFFFFFFFu, st.l0, off);
         st.l1 += __shfl_xor_sync(0xFFFFFFFFu, st.l1, off);
     }
+    if (g == 0) {
+        ml[warp][2 * c] = make_float2(st.m0, st.l0);
+        ml[warp][2 * c + 1] = make_float2(st.m1, st.l1);
+    }
     __syncthreads();  // all slots have been read
     float *merge = reinterpret_cast<float *>(smem);
     {
-        float *mine = merge + ((size_t)warp * 8 + 2 * c) * kHeadPitch + g;
+        const float unit = exp2i(st.v - 14);
+        // all maxima -infinity: no page was read, or all scores were NaN
+        auto weight = [&](int col) {
+            float M = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kWarps; w++)
+                M = fmaxf(M, ml[w][col].x);
+            return M == -INFINITY ? unit : rt::fast_exp2(ml[warp][col].x - M) * unit;
+        };
+        const float w0 = weight(2 * c), w1 = weight(2 * c + 1);
+        float *to = merge + ((size_t)warp * 8 + 2 * c) * kHeadPitch + g;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            mine[16 * i] = st.o[i][0];
-            mine[16 * i + kHeadPitch] = st.o[i][1];
-            mine[16 * i + 8] = st.o[i][2];
-            mine[16 * i + 8 + kHeadPitch] = st.o[i][3];
-        }
-        if (g == 0) {
-            ml[warp][2 * c] = make_float2(st.m0, st.l0);
-            ml[warp][2 * c + 1] = make_float2(st.m1, st.l1);
+            to[16 * i] = st.o[i][0] * w0;
+            to[16 * i + kHeadPitch] = st.o[i][1] * w1;
+            to[16 * i + 8] = st.o[i][2] * w0;
+            to[16 * i + 8 + kHeadPitch] = st.o[i][3] * w1;
         }
     }
     __syncthreads();
-    const uint32_t d = threadIdx.x;  // one dimension per thread
-    const uint64_t bh = (uint64_t)b * a.num_kv_heads + h;
-    for (uint32_t r = 0; r < G; r++) {
-        float M = -INFINITY, l = 0.0f, acc = 0.0f;
+    const uint64_t row = (uint64_t)b * H + h, slot = row * a.max_chunks + chunk;
+    for (uint32_t r = warp; r < G; r += kWarps) {  // a warp to a head, four dimensions a lane
+        float M = -INFINITY, l = 0.0f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < kWarps; w++)
             M = fmaxf(M, ml[w][r].x);
 #pragma unroll
         for (int w = 0; w < kWarps; w++) {
-            const float wt = ml[w][r].x == -INFINITY ? 0.0f : rt::fast_exp2(ml[w][r].x - M);
-            // a warp whose sum is NaN keeps it, whatever its maximum
-            l += ml[w][r].y == 0.0f ? 0.0f : ml[w][r].y * (M == -INFINITY ? 1.0f : wt);
-            acc += merge[(w * 8 + r) * kHeadPitch + d] * (M == -INFINITY ? 1.0f : wt);
+            l += ml[w][r].y * (M == -INFINITY ? 1.0f : rt::fast_exp2(ml[w][r].x - M));
+#pragma unroll
+            for (uint32_t col = r; col < 8u; col += DUP ? 4u : 8u) {
+                const float4 o = *reinterpret_cast<const float4 *>(merge + (w * 8 + col) * kHeadPitch + 4 * lane);
+                acc.x += o.x;
+                acc.y += o.y;
+                acc.z += o.z;
+                acc.w += o.w;
+            }
         }
         if (n_chunks == 1) {
-            a.out[(bh * G + r) * 128u + d] = l == 0.0f ? 0.0f : acc / l;
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            reinterpret_cast<float4 *>(a.out + (row * G + r) * 128u)[lane] =
+                make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
         } else {
-            const uint64_t slot = (bh * a.max_chunks + chunk) * G + r;
-            a.part_o[slot * 128u + d] = acc;
-            if (d == 0)
-                a.part_ml[slot] = make_float2(M, l);
+            reinterpret_cast<float4 *>(a.part_o + (slot * G + r) * 128u)[lane] = acc;
+            if (lane == 0)
+                a.part_ml[slot * G + r] = make_float2(M, l);
         }
     }
 }
 
-// Log-sum-exp merge of the chunks of sequences that have several: one warp per
-// (sequence, query head), each lane four dimensions.
-__global__ void __launch_bounds__(128) kv8_merge_kernel(const AttnArgs a)
+// Log-sum-exp merge of the chunks of sequences that have several.  It waits on
+// memory alone, so each warp has U chunks' loads in flight, a lane four dimensions
+// of each.
+//
+// WARPS = 1: one warp per (row, head), for batches of many rows.  Else one CTA per
+// (row, head), its warps taking the chunks in turn.
+template <int WARPS, int U>
+__global__ void __launch_bounds__(WARPS == 1 ? 256 : WARPS * 32) kv8_merge_kernel(const AttnArgs a)
 {
-    const int lane = threadIdx.x & 31;
-    const uint64_t row = blockIdx.x * 4ull + (threadIdx.x >> 5);
-    const uint32_t Hq = a.num_kv_heads * a.G;
-    if (row >= (uint64_t)a.num_seqs * Hq)
+    __shared__ float2 warp_ml[WARPS];
+    __shared__ float4 warp_o[WARPS][32];
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, G = a.G;
+    const uint64_t item = WARPS == 1 ? blockIdx.x * 8ull + warp : blockIdx.x;
+    if (item >= (uint64_t)a.num_seqs * a.num_kv_heads * G)
         return;
-    const uint32_t b = (uint32_t)(row / Hq), hq = (uint32_t)(row % Hq);
-    const int32_t L = a.lens[b];
+    const uint64_t row = item / G;
+    const uint32_t sub = WARPS == 1 ? 0u : warp;
+    const int32_t L = a.lens[row / a.num_kv_heads];
     if (!len_ok(a, L))
         return;
     const uint32_t n = chunks_of(a, L);
-    if (n == 1)
+    if (n < 2)
         return;
-    const uint64_t first = (((uint64_t)b * a.num_kv_heads + hq / a.G) * a.max_chunks) * a.G + hq % a.G;
-    float M = -INFINITY;
-    for (uint32_t k = lane; k < n; k += 32)
-        M = fmaxf(M, a.part_ml[first + (uint64_t)k * a.G].x);
-#pragma unroll
-    for (int off = 16; off; off >>= 1)
-        M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, off));
-    float l = 0.0f;
+    const uint64_t first = row * a.max_chunks * G + item % G;
+    rt::grid_dep_wait();
+    // all maxima -infinity: no page was read, or all scores were NaN
+    auto weight = [](float x, float top) { return top == -INFINITY ? 1.0f : rt::fast_exp2(x - top); };
+    float m = -INFINITY, l = 0.0f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (uint32_t k = 0; k < n; k++) {
-        const uint64_t slot = first + (uint64_t)k * a.G;
-        const float2 s = a.part_ml[slot];
-        const float wt = M == -INFINITY ? 1.0f : s.x == -INFINITY ? 0.0f : rt::fast_exp2(s.x - M);
-        const float4 o = reinterpret_cast<const float4 *>(a.part_o + slot * 128u)[lane];
-        l += s.y == 0.0f ? 0.0f : s.y * wt;
-        acc.x += o.x * wt;
-        acc.y += o.y * wt;
-        acc.z += o.z * wt;
-        acc.w += o.w * wt;
+    for (uint32_t k0 = sub; k0 < n; k0 += WARPS * U) {
+        float2 s[U];
+        float4 o[U];
+        float top = m;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const uint32_t k = k0 + u * WARPS;
+            s[u] = make_float2(-INFINITY, 0.0f);
+            o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (k < n) {
+                const uint64_t slot = first + (uint64_t)k * G;
+                s[u] = a.part_ml[slot];
+                o[u] = reinterpret_cast<const float4 *>(a.part_o + slot * 128u)[lane];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            top = fmaxf(top, s[u].x);
+        const float w0 = weight(m, top);
+        m = top;
+        l *= w0;
+        acc.x *= w0;
+        acc.y *= w0;
+        acc.z *= w0;
+        acc.w *= w0;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const float wt = weight(s[u].x, top);
+            l += s[u].y * wt;
+            acc.x += o[u].x * wt;
+            acc.y += o[u].y * wt;
+            acc.z += o[u].z * wt;
+            acc.w += o[u].w * wt;
+        }
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    reinterpret_cast<float4 *>(a.out + row * 128u)[lane] =
-        make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+    if constexpr (WARPS == 1) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        reinterpret_cast<float4 *>(a.out + item * 128u)[lane] =
+            make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+    } else {
+        warp_o[warp][lane] = acc;
+        if (lane == 0)
+            warp_ml[warp] = make_float2(m, l);
+        __syncthreads();
+        if (threadIdx.x < 128) {
+            float top = -INFINITY, sum = 0.0f, den = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WARPS; w++)
+                top = fmaxf(top, warp_ml[w].x);
+#pragma unroll
+            for (int w = 0; w < WARPS; w++) {
+                const float wt = weight(warp_ml[w].x, top);
+                sum += reinterpret_cast<const float *>(warp_o[w])[threadIdx.x] * wt;
+                den += warp_ml[w].y * wt;
+            }
+            a.out[item * 128u + threadIdx.x] = den == 0.0f ? 0.0f : sum / den;
+        }
+    }
 }
 
-// Pages per item: up to 64, fewer when the grid would not give every SM's slots
-// two items.
-uint32_t chunk_pages_of(const rt_kv8_attn_params_t *p)
+// Pages per item.
+struct AttnPlan {
+    uint32_t chunk_pages, max_chunks;
+    size_t part_o, part_ml;
+};
+
+AttnPlan plan_of(const rt_kv8_attn_params_t *p)
 {
-    const uint64_t pages = p->max_seq_len >> 4;
+    AttnPlan r;
+    const uint64_t rows = (uint64_t)p->num_seqs * p->num_kv_heads, pages = p->max_seq_len >> 4;
+    const uint64_t items = 3ull * kCtasPerSm * (uint64_t)rt::num_sms();
     uint64_t c = p->chunk_pages;
     if (!c) {
-        const uint64_t slots = 2ull * kCtasPerSm * (uint64_t)rt::num_sms();
-        c = (pages * p->num_seqs * p->num_kv_heads + slots - 1) / slots;
-        c = c < 8 ? 8 : c > 64 ? 64 : c;
+        c = (pages * rows + items - 1) / items;
+        c = c < 32 ? 32 : c > kMaxChunkPages ? kMaxChunkPages : c;
     }
-    return (uint32_t)c;
-}
-uint32_t max_chunks_of(const rt_kv8_attn_params_t *p, uint32_t chunk)
-{
-    const uint32_t n = ((p->max_seq_len >> 4) + chunk - 1) / chunk;
-    return n ? n : 1u;
+    r.chunk_pages = (uint32_t)((c + 1) / 2 * 2);  // whole pairs
+    r.max_chunks = (uint32_t)((pages + r.chunk_pages - 1) / r.chunk_pages);
+    r.max_chunks = r.max_chunks ? r.max_chunks : 1u;
+    const size_t parts = r.max_chunks > 1u ? (size_t)p->num_seqs * p->num_q_heads * r.max_chunks : 0u;
+    r.part_o = parts * 128u * sizeof(float);
+    r.part_ml = parts * sizeof(float2);
+    return r;
 }
 
 bool format_ok(uint32_t format) { return format == RT_KV8_E4M3 || format == RT_KV8_S8; }
@@ -678,10 +1016,8 @@ int check_attn(const rt_kv8_attn_params_t *p)
                       p->num_q_heads, p->num_kv_heads, kMaxChunkPages);
         return RT_EINVAL;
     }
-    const uint32_t chunk = chunk_pages_of(p);
-    const uint64_t items = (uint64_t)p->num_kv_heads * p->num_seqs;
-    if (items * max_chunks_of(p, chunk) > 0x7FFFFFFFull ||
-        (uint64_t)p->num_q_heads * p->num_seqs > 0x7FFFFFFFull) {
+    if ((uint64_t)p->num_q_heads * p->num_seqs > 0x7FFFFFFFull ||
+        (uint64_t)p->num_kv_heads * p->num_seqs * plan_of(p).max_chunks > 0x7FFFFFFFull) {
         rt::set_error("kv8_decode_attention: more than 2^31 - 1 work items");
         return RT_EINVAL;
     }
@@ -765,8 +1101,8 @@ extern "C" size_t rt_kv8_attn_workspace_bytes(const rt_kv8_attn_params_t *p)
 {
     if (check_attn(p) != RT_OK)
         return 0;
-    const uint32_t chunks = max_chunks_of(p, chunk_pages_of(p));
-    return chunks > 1 ? (size_t)p->num_seqs * p->num_q_heads * chunks * (128u + 2u) * 4u : 0u;
+    const AttnPlan r = plan_of(p);
+    return r.part_o + r.part_ml;
 }
 
 extern "C" int rt_kv8_decode_attention(const rt_kv8_attn_params_t *p, const void *q,
@@ -791,7 +1127,8 @@ extern "C" int rt_kv8_decode_attention(const rt_kv8_attn_params_t *p, const void
                       "aligned, scales 8-byte, the rest 4-byte");
         return RT_EINVAL;
     }
-    const size_t need = rt_kv8_attn_workspace_bytes(p);
+    const AttnPlan plan = plan_of(p);
+    const size_t need = plan.part_o + plan.part_ml;
     if (need && (!workspace || workspace_bytes < need)) {
         rt::set_error("kv8_decode_attention: workspace of %zu bytes needed, %zu given", need,
                       workspace ? workspace_bytes : (size_t)0);
@@ -813,31 +1150,41 @@ extern "C" int rt_kv8_decode_attention(const rt_kv8_attn_params_t *p, const void
     a.G = p->num_q_heads / p->num_kv_heads;
     a.max_pages = p->max_pages_per_seq;
     a.max_seq_len = p->max_seq_len;
-    a.chunk_pages = chunk_pages_of(p);
-    a.max_chunks = max_chunks_of(p, a.chunk_pages);
+    a.chunk_pages = plan.chunk_pages;
+    a.max_chunks = plan.max_chunks;
     a.scale_log2 = p->scale * 1.4426950408889634f;
-    a.part_o = static_cast<float *>(workspace);
-    a.part_ml = need ? reinterpret_cast<float2 *>(a.part_o + (size_t)p->num_seqs * p->num_q_heads *
-                                                                 a.max_chunks * 128u)
-                     : nullptr;
+    uint8_t *ws = static_cast<uint8_t *>(workspace);
+    a.part_o = reinterpret_cast<float *>(ws);
+    a.part_ml = reinterpret_cast<float2 *>(ws + plan.part_o);
     cudaStream_t s = (cudaStream_t)stream;
-    const void *fn = p->format == RT_KV8_E4M3 ? (const void *)kv8_decode_kernel<RT_KV8_E4M3>
-                                              : (const void *)kv8_decode_kernel<RT_KV8_S8>;
-    cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    void (*fn)(AttnArgs) = nullptr;
+    if (p->format == RT_KV8_E4M3)
+        fn = a.G <= 4 ? kv8_decode_kernel<RT_KV8_E4M3, true> : kv8_decode_kernel<RT_KV8_E4M3, false>;
+    else
+        fn = a.G <= 4 ? kv8_decode_kernel<RT_KV8_S8, true> : kv8_decode_kernel<RT_KV8_S8, false>;
+    cudaError_t e = cudaFuncSetAttribute((const void *)fn,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
     if (e != cudaSuccess)
         return rt::cuda_fail(e, "kv8_decode_attention: shared memory");
-    const dim3 grid(p->num_kv_heads * p->num_seqs * a.max_chunks);
-    if (p->format == RT_KV8_E4M3)
-        kv8_decode_kernel<RT_KV8_E4M3><<<grid, kWarps * 32, kSmemBytes, s>>>(a);
-    else
-        kv8_decode_kernel<RT_KV8_S8><<<grid, kWarps * 32, kSmemBytes, s>>>(a);
+    fn<<<p->num_kv_heads * p->num_seqs * plan.max_chunks, kWarps * 32, kSmemBytes, s>>>(a);
     e = cudaGetLastError();
     if (e != cudaSuccess)
         return rt::cuda_fail(e, "kv8_decode_attention: launch");
-    if (a.max_chunks > 1) {
-        const uint64_t rows = (uint64_t)p->num_seqs * p->num_q_heads;
-        kv8_merge_kernel<<<(unsigned)((rows + 3) / 4), 128, 0, s>>>(a);
-        e = cudaGetLastError();
+    if (plan.max_chunks > 1u) {
+        // a programmatic dependent: its CTAs are in place when the last items end
+        const uint32_t items = p->num_seqs * p->num_q_heads;
+        const bool many = items >= 8u * (uint32_t)rt::num_sms();
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(many ? (items + 7u) / 8u : items);
+        cfg.blockDim = dim3((many ? 8 : kMergeWarps) * 32);
+        cfg.stream = s;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        e = many ? cudaLaunchKernelEx(&cfg, kv8_merge_kernel<1, 4>, (const AttnArgs)a)
+                 : cudaLaunchKernelEx(&cfg, kv8_merge_kernel<kMergeWarps, 14>, (const AttnArgs)a);
         if (e != cudaSuccess)
             return rt::cuda_fail(e, "kv8_decode_attention: merge launch");
     }

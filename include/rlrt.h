@@ -245,11 +245,12 @@ typedef struct {
 /* Decode attention over the 8-bit cache: rt_paged_decode_attention with
  * K = scale * code.  q bf16 [num_seqs][num_q_heads][128] (rows q_stride
  * apart), out fp32 [num_seqs][num_q_heads][128]; a sequence of length 0 gives
- * zeros, one skipped for an error is left as it was.  `workspace` holds the
- * partial results of sequences that are split (0 bytes when max_seq_len fits
- * one item); it needs no initialisation, and calls that share one must not
- * overlap on the GPU.  Results do not depend on earlier calls and are the
- * same, bit for bit, in every run of a shape. */
+ * zeros, one skipped for its length is left as it was; a page skipped for its
+ * id counts as absent.  `workspace` holds the partial results of sequences that
+ * are split (none, 0 bytes, where max_seq_len is short); it needs no
+ * initialisation, and calls that share one must not overlap on the GPU.
+ * Results do not depend on earlier calls and are the same, bit for bit, in
+ * every run of the same shape on the same GPU. */
 size_t rt_kv8_attn_workspace_bytes(const rt_kv8_attn_params_t *p);
 int rt_kv8_decode_attention(const rt_kv8_attn_params_t *p, const void *q, const void *pages,
                             const float *scales, const void *tail, const int32_t *page_table,

@@ -6,10 +6,10 @@ bit.  Attention's tolerance counts the kernel's roundings.  With
 A = scale * sum_d |q_d k_d| the fp32 accumulation of a score (8 tensor-core
 steps of 16 products, each step off by at most 2^-23 of what it holds) and the
 two factors' roundings are off by at most 2^-19 A, so e^s by that share; exp2
-adds 2^-21.  P in two fp16 terms is off by 2^-22 of 1, the fp32 sums over at
-most 32 pages a warp, 4 warps and 128 chunks by 2^-24 a step: 2^-16 in all
-would be the worst case, 2^-18 covers it with the sums' roundings independent
-of one another.  Both errors enter the sum and the normaliser, hence twice:
+adds 2^-21.  P in two fp16 terms is off by 2^-22 of 1, the fp32 sums by
+2^-24 a step, of which a worker and the merge have at most some hundreds: 2^-16
+in all would be the worst case, 2^-18 covers it with the sums' roundings
+independent of one another.  Both errors enter the sum and the normaliser, hence twice:
 |error| <= 2 (2^-19 max A + 2^-18) sum_t p_t |v_t|."""
 import numpy as np
 import pytest
@@ -300,7 +300,18 @@ def test_attention_groups(pkg, cuda, fmt, heads, G):
     check(attend(pkg, cuda, *case, LENS), *case, LENS)
 
 
-@pytest.mark.parametrize("chunk", [1, 2, 3, 8, 31, 64, 128])
+@pytest.mark.parametrize("lens", [
+    [16 * 130, 16 * 37 + 5, 0, 33, 2049, 15], [7000], [16 * 64] * 3, [0, 0, 5000, 0],
+    list(range(0, 600, 7)), [20000] + [3] * 300, [161] * 150, [40000, 1, 40000, 17]])
+@pytest.mark.parametrize("heads,G", [(4, 4), (1, 8), (7, 3)])
+def test_attention_splits(pkg, cuda, lens, heads, G):
+    """Batches that are cut in every way: one row over the whole GPU, many short rows, rows
+    without tokens between, long rows beside short ones."""
+    case = make(pkg, cuda, lens, heads, G, "s8", seed=len(lens))
+    check(attend(pkg, cuda, *case, lens), *case, lens)
+
+
+@pytest.mark.parametrize("chunk", [1, 2, 3, 8, 31, 64, 127, 128])
 def test_attention_chunks(pkg, cuda, chunk):
     lens = [16 * 130, 16 * 37 + 5, 0, 33, 2049, 15]
     case = make(pkg, cuda, lens, 4, 4, "s8", seed=chunk)
@@ -441,7 +452,7 @@ def test_captured_steps_replay(pkg, cuda):
 
     def step(s, out):
         pkg.kv8_append(k, v, cu, lens, td, *s)
-        pkg.kv8_decode_attention(q, *s, td, after, max_seq_len=250, chunk_pages=4, out=out)
+        pkg.kv8_decode_attention(q, *s, td, after, max_seq_len=250, out=out)
 
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
