@@ -3,12 +3,18 @@
 // and the clipped policy loss with its gradient.  Contract: rlrt.h.
 //
 // A row is read from HBM once and its gradient written once.  A cluster of CTAs
-// holds a row in shared memory: each CTA a slice, copied there by bulk copies
-// whose pieces are reduced (running maximum, sum of exponentials, sum of
-// e^z z for the entropy) while later pieces arrive.  The slices' statistics are
-// exchanged through distributed shared memory, every CTA derives the row's
-// coefficients from them in the same order, and the gradient is computed from
-// the slice in shared memory.
+// holds a row in shared memory, each of its warps a region that it alone loads
+// (one bulk copy), reduces and turns into gradient, so regions need no barrier of
+// their own; while a row is worked on the next one's copies are under way.  The
+// warps' statistics are exchanged through distributed shared memory, one cluster
+// barrier a row; one warp of each CTA derives the row's coefficients from them,
+// in the same order everywhere.
+//
+// Exponentials are taken in base 2: with c = log2(e) / T and an integer reference
+// R, e = 2^z, z = l c - R in one fused multiply-add, whose one rounding is that of
+// a small number where e is not small (c's own rounding is a change of T by 2^-25
+// of itself, the same for all elements).  References differ between threads; sums
+// move between them by exact powers of two.
 #include <cfloat>
 #include <cmath>
 #include <cstdint>
@@ -20,13 +26,14 @@
 namespace {
 
 enum : int32_t { kErrToken = 1, kErrSeq = 2, kErrTimeout = 4 };
-constexpr int kThreads = 512;
-constexpr int kPieces = 4;
+constexpr int kCtasPerSm = 4;
+constexpr int kRowWarps = 8;
+constexpr int kThreads = kRowWarps * 32;
 constexpr uint32_t kMaxCluster = 8;
+constexpr uint32_t kMaxRows = 32;  // of a cluster or warp, one to a lane
 constexpr uint32_t kMaxVocab = 262144;
 constexpr uint64_t kWaitLimitNs = 2000000000ull;
-// Three CTAs of this much on an SM: one loads while others reduce and store.
-constexpr uint32_t kSliceTarget = 72 * 1024;
+constexpr uint32_t kSmemTarget = 72 * 1024;  // of a CTA: three to an SM
 
 struct RowArgs {
     const void *logits;
@@ -34,7 +41,8 @@ struct RowArgs {
     const uint32_t *tokens;
     int32_t *error;
     uint64_t row_stride, grad_stride;
-    uint32_t num_rows, vocab, cluster, slice;  // slice: elements per CTA, whole vectors
+    uint32_t num_rows, vocab;
+    uint32_t cluster, region, rows_each;  // region: elements of a warp, whole vectors
     float temperature;
     // log-probabilities
     const uint32_t *row_enable;
@@ -50,31 +58,36 @@ struct RowArgs {
 
 enum Mode { kForward, kBackward, kPolicy };
 
-// Running statistics of a set of logits l: their maximum m, s = sum of
-// e^((l - m) / T) and u = sum of e^((l - m) / T) (l - m).
+// Statistics of a set of logits l: an integer reference R, s = sum of 2^z and u =
+// sum of 2^z z, z = l c - R.
 struct Stats {
-    float m, s, u;
+    int R;
+    float s, u;
 };
+constexpr int kNoRef = -4194304;  // -2^22: no logit that counts is below (see kMaxRef)
+// The fused form holds while a row's reference is at most this in size, and then
+// what lies below kNoRef is 0 beside it.  Rows beyond (logits of millions, or
+// without a finite maximum) take differences to the maximum instead.
+constexpr int kMaxRef = 2097152;
 
-// The sums of a set with maximum m, for a maximum shifted by d = m - m' <= 0;
-// c = log2(e) / T.  A set without a logit above -infinity (m = -infinity, s = u =
-// 0) shifts by 0.  Where the factor is 0 the set is gone, however far it was:
-// its u is 0 and not 0 times an overflow; a NaN in s stays.
-__device__ __forceinline__ void shift(float &s, float &u, float d, float c)
+// Statistics for a reference that is higher by d.
+__device__ __forceinline__ void raise(Stats &x, int R)
 {
-    const float w = rt::fast_exp2(d * c);
-    u = w > 0.0f ? (u + s * d) * w : 0.0f;
-    s *= w;
+    const uint32_t d = (uint32_t)R - (uint32_t)x.R;
+    const float w = __int_as_float((127 - (int)min(d, 127u)) << 23);  // 2^-d, 0 from 127 on
+    x.u = w > 0.0f ? (x.u - x.s * (float)d) * w : 0.0f;
+    x.s *= w;
+    x.R = R;
 }
-__device__ __forceinline__ Stats merge(Stats a, Stats b, float c)
+// Of a warp's lanes, in all of them.
+__device__ __forceinline__ void across_warp(Stats &x)
 {
-    Stats r;
-    r.m = fmaxf(a.m, b.m);
-    shift(a.s, a.u, a.m == -INFINITY ? 0.0f : a.m - r.m, c);
-    shift(b.s, b.u, b.m == -INFINITY ? 0.0f : b.m - r.m, c);
-    r.s = a.s + b.s;
-    r.u = a.u + b.u;
-    return r;
+    raise(x, __reduce_max_sync(0xFFFFFFFFu, x.R));
+#pragma unroll
+    for (int off = 16; off; off >>= 1) {
+        x.s += __shfl_xor_sync(0xFFFFFFFFu, x.s, off);
+        x.u += __shfl_xor_sync(0xFFFFFFFFu, x.u, off);
+    }
 }
 
 __device__ __forceinline__ uint32_t cluster_rank()
@@ -91,11 +104,18 @@ __device__ __forceinline__ void cluster_wait()
 {
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void store_cluster(uint32_t addr, uint32_t rank, float v)
+// Store to the shared memory of the cluster's CTA `rank`, at the addresses that
+// `addr` and the mbarrier `bar` have here; counts 16 bytes on that mbarrier when it
+// is there.  Unlike a cluster barrier it orders nothing else, so it does not wait
+// for the gradient stores of the row before.
+__device__ __forceinline__ void send_async(uint32_t addr, uint32_t bar, uint32_t rank, uint4 v)
 {
-    uint32_t remote;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
-    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote), "f"(v) : "memory");
+    uint32_t to, to_bar;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(addr), "r"(rank));
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to_bar) : "r"(bar), "r"(rank));
+    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];"
+                 ::"r"(to), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w), "r"(to_bar)
+                 : "memory");
 }
 
 template <typename T>
@@ -115,306 +135,628 @@ __device__ __forceinline__ T from_float(float x)
         return x;
 }
 
-// One 16-byte vector of logits as floats, and back.
+// Two fp32 values in one register pair: sm_100 adds, multiplies and fuses them in
+// one instruction each.
+typedef uint64_t f32x2;
+__device__ __forceinline__ f32x2 pair(float lo, float hi)
+{
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ float2 halves(f32x2 v)
+{
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c)
+{
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b)
+{
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b)
+{
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 exp2_2(f32x2 z)
+{
+    const float2 v = halves(z);
+    return pair(rt::fast_exp2(v.x), rt::fast_exp2(v.y));
+}
+
+// Eight logits of a lane: one 16-byte vector of bf16, or two of fp32 that lie 32
+// vectors apart.  floor_of: a lower bound for them in the form that raise_to takes;
+// it lets a NaN through.
 template <typename T>
-struct Vec {
-    static constexpr int N = 16 / sizeof(T);
-    float f[N];
-    __device__ __forceinline__ void load(const uint8_t *p)
+struct Eight;
+template <>
+struct Eight<float> {
+    static constexpr int kVectors = 2;
+    typedef float Floor;
+    float4 w[2];
+    __device__ __forceinline__ void load(const uint8_t *p, bool second)
     {
-        const uint4 w = *reinterpret_cast<const uint4 *>(p);
-        const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+        w[0] = *reinterpret_cast<const float4 *>(p);
+        w[1] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        if (second)
+            w[1] = *reinterpret_cast<const float4 *>(p + 512);
+    }
+    static __device__ __forceinline__ Floor floor_of(float x) { return x; }
+    __device__ __forceinline__ void raise_to(Floor f)
+    {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if constexpr (sizeof(T) == 2) {
-                f[2 * i] = __uint_as_float(v[i] << 16);
-                f[2 * i + 1] = __uint_as_float(v[i] & 0xFFFF0000u);
-            } else {
-                f[i] = __uint_as_float(v[i]);
-            }
+        for (int i = 0; i < 2; i++) {
+            w[i].x = rt::nan_max(w[i].x, f);
+            w[i].y = rt::nan_max(w[i].y, f);
+            w[i].z = rt::nan_max(w[i].z, f);
+            w[i].w = rt::nan_max(w[i].w, f);
         }
     }
-    __device__ __forceinline__ uint4 pack() const
+    __device__ __forceinline__ float top() const
     {
-        uint32_t v[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if constexpr (sizeof(T) == 2)
-                v[i] = rt::pack_bf16x2(f[2 * i], f[2 * i + 1]);
-            else
-                v[i] = __float_as_uint(f[i]);
+        return fmaxf(fmaxf(fmaxf(w[0].x, w[0].y), fmaxf(w[0].z, w[0].w)),
+                     fmaxf(fmaxf(w[1].x, w[1].y), fmaxf(w[1].z, w[1].w)));
+    }
+    __device__ __forceinline__ f32x2 get(int i) const  // elements 2 i, 2 i + 1
+    {
+        return i & 1 ? pair(w[i >> 1].z, w[i >> 1].w) : pair(w[i >> 1].x, w[i >> 1].y);
+    }
+    __device__ __forceinline__ void set(int i, f32x2 v)
+    {
+        const float2 x = halves(v);
+        if (i & 1) {
+            w[i >> 1].z = x.x;
+            w[i >> 1].w = x.y;
+        } else {
+            w[i >> 1].x = x.x;
+            w[i >> 1].y = x.y;
         }
-        return make_uint4(v[0], v[1], v[2], v[3]);
+    }
+    __device__ __forceinline__ void store(float *p, bool second) const
+    {
+        *reinterpret_cast<float4 *>(p) = w[0];
+        if (second)
+            *reinterpret_cast<float4 *>(p + 128) = w[1];
+    }
+};
+template <>
+struct Eight<__nv_bfloat16> {
+    static constexpr int kVectors = 1;
+    typedef uint32_t Floor;
+    uint32_t w[4];
+    __device__ __forceinline__ void load(const uint8_t *p, bool)
+    {
+        const uint4 v = *reinterpret_cast<const uint4 *>(p);
+        w[0] = v.x;
+        w[1] = v.y;
+        w[2] = v.z;
+        w[3] = v.w;
+    }
+    static __device__ __forceinline__ Floor floor_of(float x)
+    {
+        const __nv_bfloat162 f = __bfloat162bfloat162(__float2bfloat16_rd(x));
+        return *reinterpret_cast<const uint32_t *>(&f);
+    }
+    static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b)
+    {
+        const __nv_bfloat162 m = __hmax2(*reinterpret_cast<const __nv_bfloat162 *>(&a),
+                                         *reinterpret_cast<const __nv_bfloat162 *>(&b));
+        return *reinterpret_cast<const uint32_t *>(&m);
+    }
+    __device__ __forceinline__ void raise_to(Floor f)
+    {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(w[i]) : "r"(f));
+    }
+    __device__ __forceinline__ float top() const
+    {
+        const uint32_t m = larger(larger(w[0], w[1]), larger(w[2], w[3]));
+        return fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xFFFF0000u));
+    }
+    __device__ __forceinline__ f32x2 get(int i) const
+    {
+        return pair(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
+    }
+    __device__ __forceinline__ void set(int i, f32x2 v)
+    {
+        const float2 x = halves(v);
+        w[i] = rt::pack_bf16x2(x.x, x.y);
+    }
+    __device__ __forceinline__ void store(__nv_bfloat16 *p, bool) const
+    {
+        *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
     }
 };
 
-// What the gradient of a row needs: dl[v] = [v = token] hit - e^((l - m) / T)
-// (q0 + q1 (l - m)).
+// What the gradient of a row needs: dl[v] = [v = token] hit - 2^z (q0 + q1 z).
 struct Gradient {
-    float hit, q0, q1;
+    float hit, q0, q1, R;
+    float m;         // exact: z = (l - m) c
+    uint32_t exact;
 };
+constexpr float kFloor = -200.0f;  // 2^z is 0 in fp32 from there on; keeps 0 times -infinity out
+constexpr double kLn2 = 0.6931471805599453;
 
-template <typename T, Mode MODE>
-__global__ void __launch_bounds__(kThreads) row_kernel(const RowArgs a)
+// ALONE: short rows, each a warp's own; no cluster, no barrier.
+template <typename T, Mode MODE, bool ALONE>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) row_kernel(const RowArgs a)
 {
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ __align__(8) uint64_t bars[kPieces];
-    __shared__ Stats warp_stats[kThreads / 32];
-    __shared__ Stats slice_stats[kMaxCluster];
-    __shared__ Gradient grad;
-    constexpr int N = Vec<T>::N;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const uint32_t rank = cluster_rank();
-    const uint32_t row = blockIdx.x / a.cluster;
-    const T *src = static_cast<const T *>(a.logits) + (uint64_t)row * a.row_stride;
-    T *dst = a.dlogits ? static_cast<T *>(a.dlogits) + (uint64_t)row * a.grad_stride : nullptr;
+    if (MODE == kPolicy)
+        rt::grid_dep_launch();
+    __shared__ __align__(8) uint64_t bars[kRowWarps];
+    __shared__ __align__(8) uint64_t sent[2];
+    // of every warp of the cluster: R, s, u, and the token's logit from its warp (else 0)
+    __shared__ uint4 stats[2][kMaxCluster * kRowWarps];
+    __shared__ Gradient grads;
+    constexpr int N = 16 / sizeof(T), kStep = 32 * N * Eight<T>::kVectors;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t rank = ALONE ? 0u : cluster_rank();
+    const uint32_t group = ALONE ? blockIdx.x * kRowWarps + (uint32_t)warp : blockIdx.x / a.cluster;
+    if (ALONE && (uint64_t)group * a.rows_each >= a.num_rows)
+        return;
+    const uint32_t row0 = group * a.rows_each;
+    const uint32_t n_rows = min(a.rows_each, a.num_rows - row0);
+    const uint32_t entry = ALONE ? 0u : rank * kRowWarps + (uint32_t)warp;
+    const uint32_t n_entries = ALONE ? 1u : a.cluster * kRowWarps;
+    const bool first = ALONE || (rank == 0 && warp == 0);  // of the row's warps
 
-    // The row from the 16-byte boundary at or before its start: `skip` elements
-    // of the first vector are not the row's.  This CTA has the vectors of
-    // [lo, hi), of which [bulk_lo, bulk_hi) are the row's in full.
-    const uint32_t skip = (uint32_t)((uintptr_t)src / sizeof(T)) % N;
-    const uint32_t end = a.vocab + skip;
-    const uint32_t lo = min(rank * a.slice, (end + N - 1) / N * N);
-    const uint32_t hi = min(lo + a.slice, (end + N - 1) / N * N);
-    const T *base = src - skip;
+    // A row in vectors from the 16-byte boundary at or before its start: `skip`
+    // elements of the first are not the row's, and the last one ends at or behind
+    // `end`.  This warp's region is [lo, hi), of which [from, to) is the row's in
+    // full vectors.
+    struct Span {
+        const T *base;
+        uint32_t skip, end, lo, hi, from, to;
+    };
+    auto span = [&](const T *row) {
+        Span r;
+        r.skip = (uint32_t)((uintptr_t)row / sizeof(T)) % N;
+        r.end = a.vocab + r.skip;
+        r.base = row - r.skip;
+        const uint32_t all = (r.end + N - 1) / N * N;
+        r.lo = min(entry * a.region, all);
+        r.hi = min(r.lo + a.region, all);
+        r.from = r.lo == 0 && r.skip ? min((uint32_t)N, r.hi) : r.lo;
+        r.to = max(r.from, min(r.hi, r.end / N * N));
+        return r;
+    };
+    auto logits_of = [&](uint32_t i) {
+        return static_cast<const T *>(a.logits) + (uint64_t)(row0 + i) * a.row_stride;
+    };
+    auto dlogits_of = [&](uint32_t i) {
+        return static_cast<T *>(a.dlogits) + (uint64_t)(row0 + i) * a.grad_stride;
+    };
 
-    const uint32_t token = a.tokens[row];
-    float weight = 1.0f;
-    uint32_t seq = row;
-    bool live = true;
-    if constexpr (MODE == kPolicy) {
-        weight = a.weights[row];
-        live = weight != 0.0f;
-        if (live && a.row_seq) {
-            seq = a.row_seq[row];
-            if (seq >= a.num_seqs) {
-                live = false;
-                if (tid == 0 && rank == 0 && a.error)
+    if (lane == 0) {
+        rt::mbar_init(rt::smem_u32(&bars[warp]), 1);
+        if (warp == 0) {
+            rt::mbar_init(rt::smem_u32(&sent[0]), 1);
+            rt::mbar_init(rt::smem_u32(&sent[1]), 1);
+        }
+        rt::mbar_fence_init();
+    }
+    __syncwarp();
+    if (!ALONE)
+        cluster_arrive();  // this CTA runs, its barriers are there: it may be sent to
+    uint8_t *here = smem + (uint32_t)warp * a.region * (uint32_t)sizeof(T);
+    T *slice = reinterpret_cast<T *>(here);
+    auto copy = [&](const Span &r) {
+        if (lane == 0 && r.from < r.to) {
+            const uint32_t bar = rt::smem_u32(&bars[warp]), bytes = (r.to - r.from) * (uint32_t)sizeof(T);
+            rt::fence_proxy_async_smem();  // a partial vector may have been stored there
+            rt::mbar_arrive_expect_tx(bar, bytes);
+            rt::bulk_load(rt::smem_u32(here) + (r.from - r.lo) * (uint32_t)sizeof(T), r.base + r.from, bytes, bar);
+        }
+    };
+    uint32_t phase = 0;
+    auto arrived = [&](const Span &r) {
+        if (r.from < r.to) {
+            if (!rt::mbar_wait_bounded(rt::smem_u32(&bars[warp]), phase, kWaitLimitNs) && a.error)
+                atomicCAS(a.error, 0, kErrTimeout);
+            phase ^= 1u;
+        }
+    };
+    // What lies in a row's partial first and last vectors is loaded by lanes: 0 .. N -
+    // 1 the first, N .. 2 N - 1 the last (a row inside one vector has it as the first).
+    auto edge_at = [&](const Span &r, uint32_t &v) {
+        v = lane < N ? (uint32_t)lane : r.end / N * N + (lane - N);
+        const bool partial = lane < N ? r.skip != 0 : lane < 2 * N && r.end % N != 0 && !(r.skip != 0 && r.end < N);
+        return partial && v >= r.lo && v < r.hi;
+    };
+    auto edge_of = [&](const Span &r) {
+        uint32_t v;
+        return edge_at(r, v) && v >= r.skip && v < r.end ? r.base[v] : from_float<T>(-INFINITY);
+    };
+
+    // Where rows are live whatever the arrays say, the first row's copy starts before
+    // they are read; one that turns out to have a bad token is waited for and dropped.
+    const bool early = MODE != kPolicy && !a.row_enable;
+    Span r = span(logits_of(0));
+    T edge = from_float<T>(0.0f);
+    auto begin = [&]() {
+        copy(r);
+        edge = edge_of(r);
+    };
+    if (early)
+        begin();
+    // Lane i knows row i of the cluster.
+    const uint32_t my_row = row0 + (uint32_t)lane;
+    uint32_t token = 0;
+    float weight = 0.0f, adv = 0.0f, old_lp = 0.0f, ref_lp = 0.0f, up_lp = 0.0f, up_h = 0.0f;
+    bool live = false, bad = false;
+    if ((uint32_t)lane < n_rows) {
+        token = a.tokens[my_row];
+        live = true;
+        if constexpr (MODE == kPolicy) {
+            weight = a.weights[my_row];
+            live = weight != 0.0f;
+            if (live) {
+                const uint32_t seq = a.row_seq ? a.row_seq[my_row] : my_row;
+                if (a.old_lp)
+                    old_lp = a.old_lp[my_row];
+                if (a.kl_coef != 0.0f)
+                    ref_lp = a.ref_lp[my_row];
+                bad = seq >= a.num_seqs;
+                if (bad && first && a.error)
                     atomicCAS(a.error, 0, kErrSeq);
+                adv = bad ? 0.0f : a.advantages[seq];
+            }
+        } else {
+            live = !a.row_enable || a.row_enable[my_row] != 0u;
+            if constexpr (MODE == kBackward) {
+                up_lp = a.dlogprobs[my_row];
+                up_h = a.dentropy ? a.dentropy[my_row] : 0.0f;
             }
         }
-    } else if (a.row_enable) {
-        live = a.row_enable[row] != 0u;
-    }
-    bool bad = false;
-    if (live && token >= a.vocab) {
-        live = false;
-        bad = true;
-        if (tid == 0 && rank == 0 && a.error)
-            atomicCAS(a.error, 0, kErrToken);
-    }
-    if (!live) {  // the same for all CTAs of the row
-        if (dst) {
-            const uint32_t from = lo > skip ? lo - skip : 0u, to = min(hi, end) - min(skip, hi);
-            for (uint32_t v = from + tid; v < to; v += kThreads)
-                dst[v] = from_float<T>(0.0f);
+        if (live && !bad && token >= a.vocab) {
+            bad = true;
+            if (first && a.error)
+                atomicCAS(a.error, 0, kErrToken);
         }
-        if (tid == 0 && rank == 0) {
+        if ((!live || bad) && first) {
             if constexpr (MODE == kPolicy) {
-                float4 *r = reinterpret_cast<float4 *>(a.rows + row);
+                float4 *r = reinterpret_cast<float4 *>(a.rows + my_row);
                 r[0] = r[1] = make_float4(0.f, 0.f, 0.f, 0.f);
             } else if (MODE == kForward && bad) {
-                a.logprobs[row] = 0.0f;
+                a.logprobs[my_row] = 0.0f;
                 if (a.entropy)
-                    a.entropy[row] = 0.0f;
+                    a.entropy[my_row] = 0.0f;
             }
         }
-        return;
+        live = live && !bad;
     }
+    const uint32_t in_range = n_rows == 32u ? 0xFFFFFFFFu : (1u << n_rows) - 1u;
+    uint32_t todo = __ballot_sync(0xFFFFFFFFu, live);  // the same in all warps of the cluster
 
-    cluster_arrive();  // this CTA runs: its shared memory may be written from now on
-    const uint32_t bulk_lo = lo == 0 && skip ? N : lo;
-    const uint32_t bulk_hi = max(bulk_lo, min(hi, end / N * N));
-    const uint32_t piece = ((bulk_hi - bulk_lo) / N + kPieces - 1) / kPieces * N;  // elements
-    auto piece_lo = [&](int k) { return min(bulk_hi, bulk_lo + k * piece); };
-    if (tid == 0) {
-#pragma unroll
-        for (int k = 0; k < kPieces; k++)
-            rt::mbar_init(rt::smem_u32(&bars[k]), 1);
-        rt::mbar_fence_init();
-#pragma unroll
-        for (int k = 0; k < kPieces; k++) {
-            const uint32_t from = piece_lo(k), n = piece_lo(k + 1) - from;
-            if (n) {
-                const uint32_t bar = rt::smem_u32(&bars[k]);
-                rt::mbar_arrive_expect_tx(bar, n * (uint32_t)sizeof(T));
-                rt::bulk_load(rt::smem_u32(smem) + (from - lo) * (uint32_t)sizeof(T), base + from,
-                              n * (uint32_t)sizeof(T), bar);
-            }
+    if (MODE != kForward && a.dlogits) {  // rows without a gradient
+        for (uint32_t none = in_range & ~todo; none; none &= none - 1) {
+            T *dst = dlogits_of(__ffs(none) - 1);
+            const Span r = span(dst);
+            T *out = dst - r.skip;
+            for (uint32_t v = r.from + lane * N; v < r.to; v += 32 * N)
+                *reinterpret_cast<uint4 *>(out + v) = make_uint4(0u, 0u, 0u, 0u);
+            for (uint32_t v = max(r.lo, r.skip) + lane; v < r.from; v += 32)
+                out[v] = from_float<T>(0.0f);
+            for (uint32_t v = r.to + lane; v < min(r.hi, r.end); v += 32)
+                out[v] = from_float<T>(0.0f);
         }
     }
-    const float l_token = to_float(src[token]);
-    // the row's partial first and last vectors, -infinity where they are not the row's
-    T *slice = reinterpret_cast<T *>(smem);
-    if (tid < 2 * N) {
-        const uint32_t v = tid < N ? (uint32_t)tid : end / N * N + (tid - N);
-        // a row inside one vector has its last vector filled as its first
-        const bool partial = tid < N ? skip != 0 : end % N != 0 && !(skip != 0 && end < N);
-        if (partial && v >= lo && v < hi)
-            slice[v - lo] = v >= skip && v < end ? base[v] : from_float<T>(-INFINITY);
-    }
-    __syncthreads();
+    uint32_t exchanges = 0;
+    if (early && !(todo & 1u))
+        arrived(r);
+    if (!ALONE)
+        cluster_wait();
+    if (!todo)
+        return;
 
     const float inv_t = a.temperature > 0.0f ? 1.0f / a.temperature : 1.0f;
     const float c = inv_t * 1.4426950408889634f;
-    Stats st{-INFINITY, 0.0f, 0.0f};
-    auto take = [&](uint32_t v) {
-        Vec<T> x;
-        x.load(smem + (size_t)(v - lo) * sizeof(T));
-        float top = x.f[0];
-#pragma unroll
-        for (int i = 1; i < N; i++)
-            top = fmaxf(top, x.f[i]);
-        if (top > st.m) {
-            shift(st.s, st.u, st.m == -INFINITY ? 0.0f : st.m - top, c);
-            st.m = top;
-        }
-        const float m = st.m == -INFINITY ? 0.0f : st.m;
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            const float d = x.f[i] - m, e = rt::fast_exp2(d * c);
-            st.s += e;
-            st.u = fmaf(e, fmaxf(d, -FLT_MAX), st.u);
-        }
-    };
-#pragma unroll
-    for (int k = 0; k < kPieces; k++) {
-        const uint32_t from = piece_lo(k), to = piece_lo(k + 1);
-        if (from < to && !rt::mbar_wait_bounded(rt::smem_u32(&bars[k]), 0, kWaitLimitNs) && a.error)
-            atomicCAS(a.error, 0, kErrTimeout);
-        for (uint32_t v = from + tid * N; v < to; v += kThreads * N)
-            take(v);
+    const float inv_c = 1.0f / c;
+    const f32x2 c2 = pair(c, c);
+    if (!(early && (todo & 1u))) {
+        r = span(logits_of(__ffs(todo) - 1));
+        begin();
     }
-    if (tid == 0 && lo < bulk_lo && lo < hi)
-        take(lo);
-    if (tid == 32 && bulk_hi < hi)
-        take(bulk_hi);
+    while (todo) {
+        const uint32_t i = __ffs(todo) - 1;
+        todo &= todo - 1;
+        {
+            uint32_t v;
+            if (edge_at(r, v))
+                slice[v - r.lo] = edge;
+        }
+        __syncwarp();
+        // The region, when it is not needed any more, is filled from the next row.
+        const Span next = todo ? span(logits_of(__ffs(todo) - 1)) : r;
+        const T next_edge = todo ? edge_of(next) : edge;
+        auto refill = [&]() {
+            __syncwarp();
+            if (todo)
+                copy(next);
+        };
+        const uint32_t hit = __shfl_sync(0xFFFFFFFFu, token, i) + r.skip;
+        float l_hit = 0.0f;  // the token's logit, in its warp
 
+        // What lies more than 200 below the reference, in base 2, is 0 in fp32 and is
+        // raised to there, which keeps 0 times -infinity out.
+        Stats st{kNoRef, 0.0f, 0.0f};
+        {
+            float limit = (float)(kNoRef + 64) * inv_c;
+            typename Eight<T>::Floor floor = Eight<T>::floor_of((float)(kNoRef - 200) * inv_c);
+            f32x2 minus_ref = pair(-(float)kNoRef, -(float)kNoRef), s2 = 0, u2 = 0;
+            arrived(r);
+#pragma unroll 1
+            for (uint32_t v = r.lo + lane * N; v < r.hi; v += kStep) {
+                Eight<T> x;
+                x.load(here + (size_t)(v - r.lo) * sizeof(T), v + 32 * N < r.hi);
+                const float top = x.top();
+                if (top > limit) {  // a reference that is a little low does no harm
+                    const float2 s = halves(s2), u = halves(u2);
+                    st.s = s.x + s.y;
+                    st.u = u.x + u.y;
+                    raise(st, __float2int_rn(top * c));
+                    s2 = pair(st.s, 0.0f);
+                    u2 = pair(st.u, 0.0f);
+                    const float ref = (float)st.R;
+                    limit = (ref + 64.0f) * inv_c;
+                    floor = Eight<T>::floor_of((ref - 200.0f) * inv_c);
+                    minus_ref = pair(-ref, -ref);
+                }
+                x.raise_to(floor);
 #pragma unroll
-    for (int off = 16; off; off >>= 1) {
-        Stats o;
-        o.m = __shfl_xor_sync(0xFFFFFFFFu, st.m, off);
-        o.s = __shfl_xor_sync(0xFFFFFFFFu, st.s, off);
-        o.u = __shfl_xor_sync(0xFFFFFFFFu, st.u, off);
-        st = merge(st, o, c);
-    }
-    if (lane == 0)
-        warp_stats[warp] = st;
-    cluster_wait();
-    __syncthreads();
-    if (warp == 0) {
-        st = lane < kThreads / 32 ? warp_stats[lane] : Stats{-INFINITY, 0.0f, 0.0f};
+                for (int j = 0; j < 4; j++) {
+                    const f32x2 z = fma2(x.get(j), c2, minus_ref), e = exp2_2(z);
+                    s2 = add2(s2, e);
+                    u2 = fma2(e, z, u2);
+                }
+            }
+            if (hit >= r.lo && hit < r.hi)
+                l_hit = to_float(slice[hit - r.lo]);
+            if (MODE == kForward || !a.dlogits)
+                refill();
+            const float2 s = halves(s2), u = halves(u2);
+            st.s = s.x + s.y;
+            st.u = u.x + u.y;
+        }
+        float l_token = 0.0f;
+        const bool leads = ALONE || warp == 0;
+        // The row's statistics in warp 0 of every CTA, the same bits in each.  Entries
+        // of one exchange land beside those of the one before; the CTA barrier behind
+        // each exchange, and that no warp sends before it, keeps a third away.
+        auto exchange = [&]() {
+            across_warp(st);
+            if constexpr (ALONE) {
+                l_token = l_hit;
+                return;
+            }
+            const uint32_t turn = exchanges & 1u, bar = rt::smem_u32(&sent[turn]);
+            if (warp == 0 && lane == 0)
+                rt::mbar_arrive_expect_tx(bar, n_entries * 16u);
+            if ((uint32_t)lane < a.cluster)
+                send_async(rt::smem_u32(&stats[turn][entry]), bar, lane,
+                           make_uint4((uint32_t)st.R, __float_as_uint(st.s), __float_as_uint(st.u),
+                                      __float_as_uint(l_hit)));
+            if (warp == 0) {
+                if (!rt::mbar_wait_bounded(bar, exchanges >> 1 & 1u, kWaitLimitNs) && a.error)
+                    atomicCAS(a.error, 0, kErrTimeout);
+                st = Stats{INT32_MIN, 0.0f, 0.0f};
+                l_token = 0.0f;
+                for (uint32_t e = lane; e < n_entries; e += 32) {
+                    const uint4 o = stats[turn][e];
+                    Stats x{(int)o.x, __uint_as_float(o.y), __uint_as_float(o.z)};
+                    const int top = max(st.R, x.R);
+                    raise(st, top);
+                    raise(x, top);
+                    st.s += x.s;
+                    st.u += x.u;
+                    l_token += __uint_as_float(o.w);
+                }
+                across_warp(st);
 #pragma unroll
-        for (int off = 16; off; off >>= 1) {
-            Stats o;
-            o.m = __shfl_xor_sync(0xFFFFFFFFu, st.m, off);
-            o.s = __shfl_xor_sync(0xFFFFFFFFu, st.s, off);
-            o.u = __shfl_xor_sync(0xFFFFFFFFu, st.u, off);
-            st = merge(st, o, c);
+                for (int off = 16; off; off >>= 1)
+                    l_token += __shfl_xor_sync(0xFFFFFFFFu, l_token, off);
+            }
+            exchanges++;
+        };
+        Gradient gr = {};
+        // Warp 0: the row's values and coefficients.
+        auto finish = [&](bool exact, float m) {
+            // the token's z, and log2 of the sum to 2^-24
+            const double z_t = exact ? ((double)l_token - (double)m) * (double)c
+                                     : (double)l_token * (double)c - (double)st.R;
+            const uint32_t bits = __float_as_uint(st.s);
+            const double log_s = st.s > 0.0f && st.s < INFINITY
+                                     ? (double)((int)(bits >> 23) - 127) +
+                                           (double)log2f(__uint_as_float((bits & 0x7FFFFFu) | 0x3F800000u))
+                                     : (double)NAN;
+            const double lp = kLn2 * (z_t - log_s);
+            const float ent = (float)(kLn2 * (log_s - (double)(st.u / st.s)));
+            float g_lp = 0.0f, g_h = 0.0f;
+            const uint32_t row = row0 + i;
+            if constexpr (MODE == kForward) {
+                if (first && lane == 0) {
+                    a.logprobs[row] = (float)lp;
+                    if (a.entropy)
+                        a.entropy[row] = ent;
+                }
+            } else if constexpr (MODE == kBackward) {
+                g_lp = __shfl_sync(0xFFFFFFFFu, up_lp, i);
+                g_h = __shfl_sync(0xFFFFFFFFu, up_h, i);
+            } else {
+                const float A = __shfl_sync(0xFFFFFFFFu, adv, i), w = __shfl_sync(0xFFFFFFFFu, weight, i);
+                const float before = __shfl_sync(0xFFFFFFFFu, old_lp, i);
+                const float ref = __shfl_sync(0xFFFFFFFFu, ref_lp, i);
+                const float ratio = a.old_lp ? expf((float)(lp - (double)before)) : 1.0f;
+                const float held = fminf(fmaxf(ratio, 1.0f - a.clip_low), 1.0f + a.clip_high);
+                const bool clipped = ratio * A > held * A;
+                const float policy = clipped ? -held * A : -ratio * A;
+                float kl = 0.0f, slope = clipped ? 0.0f : -ratio * A;
+                if (a.kl_coef != 0.0f) {
+                    const float gap = (float)((double)ref - lp), x = expm1f(gap);
+                    // e^g - 1 - g; by its series where the subtraction would lose digits
+                    kl = x - gap;
+                    if (fabsf(gap) < 0.5f)
+                        kl = gap * gap *
+                             (0.5f + gap * (1.f / 6 + gap * (1.f / 24 + gap * (1.f / 120 +
+                              gap * (1.f / 720 + gap * (1.f / 5040 + gap * (1.f / 40320)))))));
+                    slope -= a.kl_coef * x;
+                }
+                const float loss = policy + a.kl_coef * kl - a.entropy_coef * ent;
+                g_lp = slope * w;
+                g_h = -a.entropy_coef * w;
+                if (first && lane == 0) {
+                    float4 *to = reinterpret_cast<float4 *>(a.rows + row);
+                    to[0] = make_float4((float)lp, ent, loss, policy);
+                    to[1] = make_float4(kl, ratio, clipped ? 1.0f : 0.0f, w);
+                }
+            }
+            // 2^z / s (g_lp + g_h (log p + H)) / T, log p = ln 2 (z - log2 s)
+            const float scale = inv_t / st.s;
+            gr.hit = g_lp * inv_t;
+            gr.q0 = scale * (g_lp + g_h * (ent - (float)(kLn2 * log_s)));
+            gr.q1 = scale * g_h * (float)kLn2;
+            gr.R = (float)st.R;
+            gr.m = m;
+            gr.exact = exact ? 1u : 0u;
+            if (!ALONE && lane == 0)
+                grads = gr;
+        };
+        // What warp 0 has written to grads, in all warps.
+        auto share = [&]() {
+            if constexpr (!ALONE) {
+                __syncthreads();
+                gr = grads;
+            }
+        };
+        exchange();
+        if (leads) {
+            if (st.R > kNoRef && st.R <= kMaxRef) {
+                finish(false, 0.0f);
+            } else {
+                gr.exact = 1u;
+                if (!ALONE && lane == 0)
+                    grads = gr;
+            }
         }
-        if ((uint32_t)lane < a.cluster) {
-            const uint32_t at = rt::smem_u32(&slice_stats[rank]);
-            store_cluster(at, lane, st.m);
-            store_cluster(at + 4, lane, st.s);
-            store_cluster(at + 8, lane, st.u);
+        share();
+        if (gr.exact) {  // once more, with differences to the maximum
+            // from memory: the region may hold the next row already
+            const uint32_t v0 = max(r.lo, r.skip) + lane, v1 = min(r.hi, r.end);
+            float m = -INFINITY;
+            for (uint32_t v = v0; v < v1; v += 32)
+                m = fmaxf(m, to_float(r.base[v]));
+            // bits whose order as integers is the floats'
+            auto ordered = [](float x) {
+                const int b = __float_as_int(x);
+                return b ^ (b >> 31 & 0x7FFFFFFF);
+            };
+            st = Stats{__reduce_max_sync(0xFFFFFFFFu, ordered(m)), 0.0f, 0.0f};
+            exchange();
+            if (leads) {
+                gr.m = __int_as_float(st.R ^ (st.R >> 31 & 0x7FFFFFFF));
+                if (!ALONE && lane == 0)
+                    grads = gr;
+            }
+            share();
+            m = gr.m;
+            st = Stats{0, 0.0f, 0.0f};
+            f32x2 s2 = 0, u2 = 0;
+            for (uint32_t v = v0; v < v1; v += 64) {
+                const float y = v + 32 < v1 ? to_float(r.base[v + 32]) - m : -INFINITY;
+                const f32x2 z = pair(rt::nan_max((to_float(r.base[v]) - m) * c, kFloor),
+                                     rt::nan_max(y * c, kFloor));
+                const f32x2 e = exp2_2(z);
+                s2 = add2(s2, e);
+                u2 = fma2(e, z, u2);
+            }
+            st.s = halves(s2).x + halves(s2).y;
+            st.u = halves(u2).x + halves(u2).y;
+            exchange();
+            if (leads)
+                finish(true, m);
+            share();
         }
-    }
-    cluster_arrive();
-    cluster_wait();
 
-    if (tid == 0) {
-        st = slice_stats[0];
-        for (uint32_t k = 1; k < a.cluster; k++)
-            st = merge(st, slice_stats[k], c);
-        const double inv_td = a.temperature > 0.0f ? 1.0 / (double)a.temperature : 1.0;
-        const double log_s = log((double)st.s);
-        const double lp = ((double)l_token - (double)st.m) * inv_td - log_s;
-        const double ent = log_s - (double)st.u / (double)st.s * inv_td;
-        double g_lp = 0.0, g_h = 0.0;
-        if constexpr (MODE == kForward) {
-            if (rank == 0) {
-                a.logprobs[row] = (float)lp;
-                if (a.entropy)
-                    a.entropy[row] = (float)ent;
-            }
-        } else if constexpr (MODE == kBackward) {
-            g_lp = a.dlogprobs[row];
-            g_h = a.dentropy ? a.dentropy[row] : 0.0f;
-        } else {
-            const double adv = a.advantages[seq];
-            const double ratio = a.old_lp ? exp(lp - (double)a.old_lp[row]) : 1.0;
-            const double held = fmin(fmax(ratio, 1.0 - (double)a.clip_low), 1.0 + (double)a.clip_high);
-            const bool clipped = ratio * adv > held * adv;
-            const double policy = clipped ? -held * adv : -ratio * adv;
-            double kl = 0.0, slope = clipped ? 0.0 : -ratio * adv;
-            if (a.kl_coef != 0.0f) {
-                const double gap = (double)a.ref_lp[row] - lp, x = expm1(gap);
-                kl = x - gap;
-                slope -= (double)a.kl_coef * x;
-            }
-            const double loss = policy + (double)a.kl_coef * kl - (double)a.entropy_coef * ent;
-            g_lp = slope * (double)weight;
-            g_h = -(double)a.entropy_coef * (double)weight;
-            if (rank == 0) {
-                float4 *r = reinterpret_cast<float4 *>(a.rows + row);
-                r[0] = make_float4((float)lp, (float)ent, (float)loss, (float)policy);
-                r[1] = make_float4((float)kl, (float)ratio, clipped ? 1.0f : 0.0f, weight);
-            }
-        }
-        // e / s (g_lp + g_h (log p + H)) / T, log p = (l - m) / T - log s
-        const double scale = inv_td / (double)st.s;
-        grad.hit = (float)(g_lp * inv_td);
-        grad.q0 = (float)(scale * (g_lp + g_h * (ent - log_s)));
-        grad.q1 = (float)(scale * g_h * inv_td);
-        warp_stats[0].m = st.m;
-    }
-    if (MODE == kForward || !dst)
-        return;
-    __syncthreads();
-    const Gradient gr = grad;
-    const float m = warp_stats[0].m;
-    const float floor_d = -200.0f / c;  // e^(d / T) is 0 in fp32 from there on
-    auto slope = [&](float l) {
-        const float d = fmaxf(l - m, floor_d);
-        return -rt::fast_exp2(d * c) * fmaf(gr.q1, d, gr.q0);
-    };
-    const uint32_t hit = token + skip;
-    const uint32_t dskip = (uint32_t)((uintptr_t)dst / sizeof(T)) % N;
-    if (dskip == skip) {
-        T *out = dst - skip;
-        for (uint32_t v = bulk_lo + tid * N; v < bulk_hi; v += kThreads * N) {
-            Vec<T> x;
-            x.load(smem + (size_t)(v - lo) * sizeof(T));
+        if (MODE != kForward && a.dlogits) {
+            auto slope = [&](uint32_t v) {
+                const float l = to_float(slice[v - r.lo]);
+                const float z = fmaxf(gr.exact ? (l - gr.m) * c : fmaf(l, c, -gr.R), kFloor);
+                return from_float<T>((v == hit ? gr.hit : 0.0f) - rt::fast_exp2(z) * fmaf(gr.q1, z, gr.q0));
+            };
+            T *dst = dlogits_of(i), *out = dst - r.skip;
+            if ((uint32_t)((uintptr_t)dst / sizeof(T)) % N == r.skip && !gr.exact) {
+                const f32x2 minus_ref = pair(-gr.R, -gr.R);
+                const f32x2 minus_q0 = pair(-gr.q0, -gr.q0), minus_q1 = pair(-gr.q1, -gr.q1);
+                const typename Eight<T>::Floor floor = Eight<T>::floor_of((gr.R - 200.0f) * inv_c);
+                {  // the partial vectors at the row's ends
+                    uint32_t v;
+                    if (edge_at(r, v) && v >= r.skip && v < r.end)
+                        out[v] = slope(v);
+                }
+                if (gr.q1 != 0.0f) {
+#pragma unroll 1
+                    for (uint32_t v = r.from + lane * N; v < r.to; v += kStep) {
+                        Eight<T> x;
+                        x.load(here + (size_t)(v - r.lo) * sizeof(T), v + 32 * N < r.to);
+                        x.raise_to(floor);
 #pragma unroll
-            for (int i = 0; i < N; i++)
-                x.f[i] = slope(x.f[i]);
-            if (hit - v < (uint32_t)N) {
+                        for (int j = 0; j < 4; j++) {
+                            const f32x2 z = fma2(x.get(j), c2, minus_ref);
+                            x.set(j, mul2(exp2_2(z), fma2(minus_q1, z, minus_q0)));
+                        }
+                        x.store(out + v, v + 32 * N < r.to);
+                    }
+                } else {  // no entropy term
+#pragma unroll 1
+                    for (uint32_t v = r.from + lane * N; v < r.to; v += kStep) {
+                        Eight<T> x;
+                        x.load(here + (size_t)(v - r.lo) * sizeof(T), v + 32 * N < r.to);
 #pragma unroll
-                for (int i = 0; i < N; i++)
-                    x.f[i] += v + i == hit ? gr.hit : 0.0f;
+                        for (int j = 0; j < 4; j++)
+                            x.set(j, mul2(exp2_2(fma2(x.get(j), c2, minus_ref)), minus_q0));
+                        x.store(out + v, v + 32 * N < r.to);
+                    }
+                }
+                // the token, by the lane that has stored its vector
+                if (hit >= r.from && hit < r.to && (uint32_t)lane == (hit - r.from) / N % 32u)
+                    out[hit] = slope(hit);
+                refill();
+            } else {
+                for (uint32_t v = max(r.lo, r.skip) + lane; v < min(r.hi, r.end); v += 32)
+                    out[v] = slope(v);
+                refill();
             }
-            *reinterpret_cast<uint4 *>(out + v) = x.pack();
         }
-        // the partial vectors at the row's ends
-        if (tid < 2 * N) {
-            const uint32_t v = tid < N ? lo + tid : bulk_hi + (tid - N);
-            const bool mine = tid < N ? v < bulk_lo : v >= bulk_lo;
-            if (mine && v < hi && v >= skip && v < end)
-                out[v] = from_float<T>(slope(to_float(slice[v - lo])) + (v == hit ? gr.hit : 0.0f));
-        }
-    } else {
-        for (uint32_t v = max(lo, skip) + tid; v < min(hi, end); v += kThreads)
-            dst[v - skip] = from_float<T>(slope(to_float(slice[v - lo])) + (v == hit ? gr.hit : 0.0f));
+        r = next;
+        edge = next_edge;
     }
 }
 
-// Weighted sums over the rows' records, in fp64 and a fixed order.
-__global__ void __launch_bounds__(1024) policy_stats_kernel(const rt_policy_row_t *rows, uint32_t n,
-                                                            float *stats)
+// Weighted sums over the rows' records, in fp64 and a fixed order: one cluster of
+// CTAs, each an equal share of the rows, the shares' sums added by the first CTA.
+constexpr uint32_t kStatsCtas = 8;
+__global__ void __launch_bounds__(512) policy_stats_kernel(const rt_policy_row_t *rows, uint32_t n,
+                                                           float *stats)
 {
-    __shared__ double part[32][5];
+    __shared__ double part[16][5];
+    __shared__ double shares[kStatsCtas][5];
+    const uint32_t rank = blockIdx.x;
+    cluster_arrive();
+    rt::grid_dep_wait();  // the rows' records are there
     double sum[5] = {0, 0, 0, 0, 0};
-    for (uint32_t r = threadIdx.x; r < n; r += 1024) {
+    for (uint32_t r = rank * 512u + threadIdx.x; r < n; r += kStatsCtas * 512u) {
         const float4 x = reinterpret_cast<const float4 *>(rows + r)[0];
         const float4 y = reinterpret_cast<const float4 *>(rows + r)[1];
         const double w = y.w;
@@ -434,41 +776,48 @@ __global__ void __launch_bounds__(1024) policy_stats_kernel(const rt_policy_row_
         if ((threadIdx.x & 31) == 0)
             part[threadIdx.x >> 5][i] = sum[i];
     }
+    cluster_wait();  // the first CTA runs
     __syncthreads();
     if (threadIdx.x < 5) {
         double s = 0.0;
-        for (int w = 0; w < 32; w++)
+        for (int w = 0; w < 16; w++)
             s += part[w][threadIdx.x];
+        uint32_t to;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, 0;"
+                     : "=r"(to) : "r"(rt::smem_u32(&shares[rank][threadIdx.x])));
+        asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(to), "d"(s) : "memory");
+    }
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+    if (rank == 0 && threadIdx.x < 5) {
+        double s = 0.0;
+        for (uint32_t k = 0; k < kStatsCtas; k++)
+            s += shares[k][threadIdx.x];
         stats[threadIdx.x] = (float)s;
     }
 }
 
-// CTAs to a row: as few as make a slice fit the target, then more while the
-// rows would leave SMs idle and a slice keeps 8 KiB.
-template <typename T, Mode MODE>
-int launch_rows(RowArgs &a, cudaStream_t stream, const char *what)
+// Short rows, when there are enough of them for all SMs' warps, are a warp's own.
+// Else CTAs to a row: as few as make a slice fit the target, then more while the
+// rows would leave SMs idle and a slice keeps 8 KiB.  A group (a cluster or a warp)
+// takes several rows, so that the next row's copy starts as each warp ends its part
+// of the last: all groups at once where that makes a few rows each, so that no
+// group starts late; blocks of 8 where there are many, which the hardware balances
+// (8,192 rows of 32,000 fp32: 351 us, one row to a group 380).
+template <typename T, Mode MODE, bool ALONE>
+int launch_rows(RowArgs &a, uint32_t k, cudaStream_t stream, const char *what)
 {
-    const uint32_t N = Vec<T>::N, esz = sizeof(T);
-    auto slice_of = [&](uint32_t k) { return ((a.vocab + N - 1 + k - 1) / k + N - 1) / N * N; };
-    uint32_t k = 1;
-    while (k < kMaxCluster && (uint64_t)slice_of(k) * esz > kSliceTarget)
-        k *= 2;
-    const uint64_t slots = 2ull * (uint64_t)rt::num_sms();
-    while (k < kMaxCluster && (uint64_t)a.num_rows * k * 2 <= slots && slice_of(2 * k) * esz >= 8192)
-        k *= 2;
+    const uint32_t N = 16 / sizeof(T), esz = sizeof(T);
+    const uint32_t warps = ALONE ? 1u : k * kRowWarps, groups = ALONE ? kRowWarps : 1u;
     a.cluster = k;
-    a.slice = slice_of(k);
-    if ((uint64_t)a.num_rows * k > 0x7FFFFFFFull) {
-        rt::set_error("%s: too many rows (%u)", what, a.num_rows);
-        return RT_EINVAL;
-    }
-    const size_t bytes = (size_t)a.slice * esz;
-    cudaError_t e = cudaFuncSetAttribute(row_kernel<T, MODE>,
+    a.region = ((a.vocab + N - 1 + N - 1) / N + warps - 1) / warps * N;
+    const uint32_t one = a.region * kRowWarps * esz;
+    const size_t bytes = (size_t)one;
+    cudaError_t e = cudaFuncSetAttribute(row_kernel<T, MODE, ALONE>,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-    if (e != cudaSuccess)
-        return rt::cuda_fail(e, what);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(a.num_rows * k);
+    cfg.gridDim = dim3(k);
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = bytes;
     cfg.stream = stream;
@@ -478,15 +827,46 @@ int launch_rows(RowArgs &a, cudaStream_t stream, const char *what)
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, row_kernel<T, MODE>, (const RowArgs)a);
+    int fit = 0;
+    if (e == cudaSuccess)
+        e = cudaOccupancyMaxActiveClusters(&fit, row_kernel<T, MODE, ALONE>, &cfg);
+    if (e != cudaSuccess)
+        return rt::cuda_fail(e, what);
+    const uint64_t at_once = (uint64_t)(fit > 0 ? fit : 1) * groups;
+    uint64_t each = ((uint64_t)a.num_rows + at_once - 1) / at_once;
+    if (!ALONE && each > 24)
+        each = 8;
+    a.rows_each = (uint32_t)(each > kMaxRows ? kMaxRows : each);
+    const uint64_t in_groups = ((uint64_t)a.num_rows + a.rows_each - 1) / a.rows_each;
+    const uint64_t ctas = (in_groups + groups - 1) / groups * k;
+    if (ctas > 0x7FFFFFFFull) {
+        rt::set_error("%s: too many rows (%u)", what, a.num_rows);
+        return RT_EINVAL;
+    }
+    cfg.gridDim = dim3((unsigned)ctas);
+    e = cudaLaunchKernelEx(&cfg, row_kernel<T, MODE, ALONE>, (const RowArgs)a);
     return e == cudaSuccess ? RT_OK : rt::cuda_fail(e, what);
+}
+
+template <typename T, Mode MODE>
+int launch_shape(RowArgs &a, cudaStream_t stream, const char *what)
+{
+    const uint64_t row = (uint64_t)a.vocab * sizeof(T) + 16u, sms = (uint64_t)rt::num_sms();
+    if (a.vocab <= 6000u && a.num_rows >= 4u * sms)
+        return launch_rows<T, MODE, true>(a, 1u, stream, what);
+    uint32_t k = 1;
+    while (k < kMaxCluster && row > (uint64_t)k * kSmemTarget)
+        k *= 2;
+    while (k < kMaxCluster && a.num_rows * 2ull * k <= kCtasPerSm * sms && row / (2 * k) >= 8192)
+        k *= 2;
+    return launch_rows<T, MODE, false>(a, k, stream, what);
 }
 
 template <Mode MODE>
 int launch_typed(RowArgs &a, uint32_t dtype, cudaStream_t stream, const char *what)
 {
-    return dtype == RT_DTYPE_BF16 ? launch_rows<__nv_bfloat16, MODE>(a, stream, what)
-                                  : launch_rows<float, MODE>(a, stream, what);
+    return dtype == RT_DTYPE_BF16 ? launch_shape<__nv_bfloat16, MODE>(a, stream, what)
+                                  : launch_shape<float, MODE>(a, stream, what);
 }
 
 // Arguments that all entry points share.
@@ -656,7 +1036,20 @@ extern "C" int rt_policy_loss(const rt_policy_params_t *p, const void *logits,
         if (rc2 != RT_OK)
             return rc2;
     }
-    policy_stats_kernel<<<1, 1024, 0, s>>>(rows, p->num_rows, stats);
-    const cudaError_t e = cudaGetLastError();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(kStatsCtas);
+    cfg.blockDim = dim3(512);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = kStatsCtas;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    // in place when the last rows end
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, policy_stats_kernel, (const rt_policy_row_t *)rows,
+                                             p->num_rows, stats);
     return e == cudaSuccess ? RT_OK : rt::cuda_fail(e, "policy_loss: stats launch");
 }

@@ -2,15 +2,16 @@
 rt_token_logprobs_backward, rt_policy_loss) against plain 64-bit
 implementations.
 
-Tolerances count the kernels' roundings.  A thread adds at most 64
+Tolerances count the kernels' roundings.  A thread adds at most 72
 exponentials and merges them with the others' in at most 20 steps, each off by
 2^-24; an exponential is off by 2^-22 (exp2) and by the share 2^-22 d of its
 exponent's roundings, with d e^-d <= 0.37.  So the relative error of the sum is
-at most E = 2^-22 + 0.37 x 2^-22 + 84 x 2^-24 < 6e-6: the log-probability is
+at most E = 2^-22 + 0.37 x 2^-22 + 92 x 2^-24 < 6e-6: the log-probability is
 off by E + 2^-24 |lp|, the entropy by E (1 + sum p |d|) + 2^-24 H, and an
 element of the gradient, with the coefficient's own error from lp, by
 p |coefficient| (2 E + 2^-22 |d|) + 2^-23 of what is added, + half a step of its
-type.  An exponent of the policy loss magnifies lp's error by its own value."""
+type.  Where log p and H cancel (a vocabulary of one: both are 0) their own
+errors stay: p |dentropy| (E + E (1 + sum p |d|)) more.  An exponent of the policy loss magnifies lp's error by its own value."""
 import math
 
 import pytest
@@ -39,7 +40,9 @@ def grad64(p, logp, d, h, tokens, g, gh, t, dtype):
     inner = g[:, None] + gh[:, None] * (logp + h[:, None])
     ref = -p * inner
     size = p * (g.abs()[:, None] + gh.abs()[:, None] * (logp.abs() + h.abs()[:, None]))
+    spread = (p * torch.where(p == 0, 0.0, d).abs()).sum(1)
     off = size * (2 * E + 2.0 ** -22 * torch.where(p == 0, 0.0, d).abs())
+    off += p * (gh.abs() * E * (2 + spread))[:, None]
     hit = tokens.long()[:, None]
     ref.scatter_add_(1, hit, g[:, None])
     off.scatter_add_(1, hit, g.abs()[:, None] * 2.0 ** -23)
@@ -78,7 +81,8 @@ def check_backward(pkg, logits, tokens, t, seed=0, **kw):
 
 
 SIZES = [(1, 1), (3, 2), (5, 3), (2, 7), (4, 8), (3, 9), (1, 15), (33, 100), (7, 1001), (300, 4097),
-         (2, 32000), (700, 32000), (5, 50001), (3, 131077), (2, 262144)]
+         (2, 32000), (700, 32000), (5, 50001), (3, 131077), (2, 262144),
+         (700, 1), (1500, 37), (9000, 100), (2000, 1001), (640, 2290), (600, 4500), (1000, 8191)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
@@ -177,7 +181,58 @@ def test_logprobs_rows_skipped_and_bad_tokens(pkg, cuda):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("R,V", [(5, 1003), (400, 32000), (2, 200000)])
+@pytest.mark.parametrize("R,V", [(900, 555), (60, 20011)])
+def test_logprobs_awkward_rows_among_others(pkg, cuda, R, V, dtype):
+    """Rows without a number, masked rows, rows of logits in the millions (of which one at the
+    top of the fp32 range), skipped rows and bad tokens, each beside ordinary ones; short rows
+    and long ones, at odd strides."""
+    logits, tokens = logits_of(cuda, R, V, dtype, 31, offset=1, stride=V + 2)
+    low = torch.finfo(dtype).min
+    for r in range(R):
+        kind = r % 10
+        if kind == 0:
+            logits[r, r % V] = math.nan
+        elif kind == 1:
+            logits[r, r % V] = math.inf
+        elif kind == 2:
+            logits[r] = -math.inf
+        elif kind == 3:
+            logits[r] = low
+        elif kind == 4:
+            logits[r] *= 3e6
+        elif kind == 5:
+            logits[r, : V // 2] = low
+        elif kind == 6:
+            logits[r] = logits[r] * 1e3 - 1e30
+        elif kind == 7:
+            logits[r, 0] = 3e38
+    tokens[8::10] = V
+    enable = torch.ones(R, dtype=torch.int32, device=cuda)
+    enable[9::20] = 0
+    error = torch.zeros(1, dtype=torch.int32, device=cuda)
+    lp, h = torch.full((R,), 9.0, device=cuda), torch.full((R,), 9.0, device=cuda)
+    pkg.token_logprobs(logits, tokens, row_enable=enable, logprobs=lp, entropy=h, error=error)
+    assert error.item() == 1
+    one = torch.ones(R, device=cuda)
+    grad = pkg.token_logprobs_backward(logits, tokens, one, one, row_enable=enable)
+    at = torch.arange(R, device=cuda)
+    bad, off = at % 10 == 8, at % 20 == 9
+    assert bool((lp[bad] == 0).all()) and bool((h[bad] == 0).all())
+    assert bool((lp[off] == 9).all()) and bool((h[off] == 9).all())
+    assert bool((grad[bad | off] == 0).all())
+    p, logp, d, want, ent, spread = rows64(logits, tokens.clamp(max=V - 1), 1.0)
+    nan = (at % 10 < 3) & ~bad & ~off
+    assert bool(torch.isnan(lp[nan]).all()) and bool(torch.isnan(h[nan]).all())
+    assert bool(torch.isnan(grad[nan]).all())
+    ok = ~nan & ~bad & ~off
+    assert bool(((lp[ok].double() - want[ok]).abs() <= E + 2.0 ** -24 * want[ok].abs()).all())
+    assert bool(((h[ok].double() - ent[ok]).abs() <= E * (1 + spread[ok]) + 2.0 ** -24 * ent[ok]).all())
+    ref, tol = grad64(p, logp, d, ent, tokens.clamp(max=V - 1), one.double(), one.double(), 1.0, dtype)
+    assert bool(((grad[ok].double() - ref[ok]).abs() <= tol[ok]).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("R,V", [(700, 300), (5, 1003), (400, 32000), (2, 200000)])
 def test_gradient_in_place(pkg, cuda, R, V, dtype):
     logits, tokens = logits_of(cuda, R, V, dtype, 9)
     g = torch.linspace(-1, 1, R, device=cuda)
@@ -254,7 +309,7 @@ def check_policy(pkg, c, t=1.0, lo=0.2, hi=0.2, kl=0.04, ent=0.01, **kw):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("R,V,groups", [(1, 1, None), (3, 17, None), (64, 1000, 4), (33, 32001, 5),
-                                        (600, 32000, 75), (3, 131072, None)])
+                                        (600, 32000, 75), (3, 131072, None), (3000, 601, 30)])
 def test_policy_sizes(pkg, cuda, dtype, R, V, groups):
     check_policy(pkg, case(cuda, R, V, dtype, R + V, groups), t=0.8)
 
