@@ -34,7 +34,7 @@ struct AppendArgs {
     int32_t *error;
     uint64_t k_stride, v_stride, arena_pages;
     uint32_t num_seqs, num_kv_heads, num_tokens, max_pages;
-    uint64_t n_warps;  // units x heads x 2 planes
+    uint64_t n_items;  // units x KV heads
 };
 
 constexpr int kAppendWarps = 8;
@@ -51,42 +51,129 @@ __device__ __forceinline__ uint2 load4(const void *base, uint64_t elem)
     }
 }
 
+__device__ __forceinline__ float bf16_lo(uint32_t v) { return __uint_as_float(v << 16); }
+__device__ __forceinline__ float bf16_hi(uint32_t v) { return __uint_as_float(v & 0xFFFF0000u); }
+
+// Codes of two quotients, in the two low bytes; the others hold anything.
 template <uint32_t FMT>
-__device__ __forceinline__ uint32_t quantise4(uint2 x, float scale)
+__device__ __forceinline__ uint32_t codes2(rt::f32x2 y)
 {
-    const float f[4] = {__uint_as_float(x.x << 16), __uint_as_float(x.x & 0xFFFF0000u),
-                        __uint_as_float(x.y << 16), __uint_as_float(x.y & 0xFFFF0000u)};
-    float y[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-        y[i] = __fdiv_rn(f[i], scale);
     if constexpr (FMT == RT_KV8_E4M3) {
-        uint16_t lo, hi;
-        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(y[1]), "f"(y[0]));
-        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(y[3]), "f"(y[2]));
-        return (uint32_t)lo | (uint32_t)hi << 16;
+        const float2 v = rt::halves(y);
+        uint16_t r;
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(v.y), "f"(v.x));
+        return r;
     } else {
-        uint32_t w = 0;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int c = __float2int_rn(fminf(fmaxf(y[i], -127.0f), 127.0f));
-            w |= ((uint32_t)c & 0xFFu) << (8 * i);
-        }
-        return w;
+        // 1.5 x 2^23 + y rounds y to the nearest integer, ties to even, and holds it in
+        // its low bits
+        constexpr float kRound = 12582912.0f;
+        const float2 v = rt::halves(rt::add2(y, rt::pair(kRound, kRound)));
+        return __byte_perm(__float_as_uint(v.x), __float_as_uint(v.y), 0x0040);
     }
 }
 
-// One warp per (unit, KV head, plane); a unit is one page of one sequence that
+// Codes of four elements.  The quotient has to be the correctly rounded one, since
+// codes change at quotients of k + 1/2: with inv the correctly rounded reciprocal,
+// q = x inv and one step q + (x - q scale) inv, in fused operations, give it
+// (Markstein, IBM J. Res. Dev. 34, 1990), as long as nothing leaves the normal
+// range; tiles of other scales divide.
+template <uint32_t FMT>
+__device__ __forceinline__ uint32_t quantise4(uint2 x, float scale, float inv, bool plain)
+{
+    const uint32_t w[2] = {x.x, x.y};
+    uint32_t r[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const float lo = bf16_lo(w[i]), hi = bf16_hi(w[i]);
+        if (plain) {
+            const rt::f32x2 f = rt::pair(lo, hi), inv2 = rt::pair(inv, inv);
+            const rt::f32x2 q = rt::mul2(f, inv2);
+            r[i] = codes2<FMT>(rt::fma2(rt::fma2(q, rt::pair(-scale, -scale), f), inv2, q));
+        } else {
+            const float most = FMT == RT_KV8_E4M3 ? 448.0f : 127.0f;
+            r[i] = codes2<FMT>(rt::pair(fminf(fmaxf(__fdiv_rn(lo, scale), -most), most),
+                                        fminf(fmaxf(__fdiv_rn(hi, scale), -most), most)));
+        }
+    }
+    return __byte_perm(r[0], r[1], 0x5410);
+}
+
+// Word w of a tile in shared memory: 16-byte vectors are permuted among the 8 of a
+// 128-byte row so that the scattered word stores below meet few bank conflicts (K
+// two ways, V none) and the vectors are read back without any.
+__device__ __forceinline__ uint32_t staged(uint32_t w)
+{
+    return w ^ (((w >> 7) << 1 | (w >> 6 & 1u)) << 2);
+}
+
+// Quantise one tile (lane: dimensions 4 lane .. 4 lane + 3 of the 16 tokens) and
+// store it in page order.
+template <uint32_t FMT>
+__device__ __forceinline__ void store_tile(const uint2 (&x)[16], uint32_t plane, uint32_t *stage,
+                                           uint8_t *page, float *scale_out)
+{
+    const uint32_t lane = threadIdx.x & 31;
+    uint32_t top2 = 0;  // per 16-bit half: the largest magnitude's bits
+#pragma unroll
+    for (int t = 0; t < 16; t++)
+        top2 = __vmaxu2(top2, __vmaxu2(x[t].x & 0x7FFF7FFFu, x[t].y & 0x7FFF7FFFu));
+    const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, max(top2 & 0xFFFFu, top2 >> 16));
+    // a NaN's or infinity's bits are above every number's
+    const float scale = top >= 0x7F80u ? __int_as_float(0x7FC00000)
+                                       : __fdiv_rn(__uint_as_float(top << 16),
+                                                   FMT == RT_KV8_E4M3 ? 448.0f : 127.0f);
+    const bool plain = scale > 0x1p-90f && scale < 0x1p90f;
+    const float inv = plain ? __frcp_rn(scale) : 0.0f;
+    uint32_t w[16];
+    if (plain) {
+#pragma unroll
+        for (int t = 0; t < 16; t++)
+            w[t] = quantise4<FMT>(x[t], scale, inv, true);
+    } else {
+#pragma unroll
+        for (int t = 0; t < 16; t++)
+            w[t] = scale > 0.0f ? quantise4<FMT>(x[t], scale, 0.0f, false) : 0u;
+    }
+    if (plane == 0) {
+#pragma unroll
+        for (int t = 0; t < 16; t++)
+            stage[staged(rt_kv8_k_offset(t, 4 * lane) / 4)] = w[t];
+    } else {
+        // words of tokens {2c, 2c+1, 2c+8, 2c+9} x 4 dimensions -> 4 words of 4 tokens
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            const uint32_t r0 = w[2 * c], r1 = w[2 * c + 1], r2 = w[2 * c + 8], r3 = w[2 * c + 9];
+            const uint32_t p0 = __byte_perm(r0, r1, 0x5140), p1 = __byte_perm(r0, r1, 0x7362);
+            const uint32_t q0 = __byte_perm(r2, r3, 0x5140), q1 = __byte_perm(r2, r3, 0x7362);
+            const uint32_t o[4] = {__byte_perm(p0, q0, 0x5410), __byte_perm(p0, q0, 0x7632),
+                                   __byte_perm(p1, q1, 0x5410), __byte_perm(p1, q1, 0x7632)};
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                stage[staged(rt_kv8_v_offset(2 * c, 4 * lane + e) / 4)] = o[e];
+        }
+    }
+    __syncwarp();
+    uint4 *dst = reinterpret_cast<uint4 *>(page);
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        dst[i * 32 + lane] = *reinterpret_cast<const uint4 *>(stage + staged((i * 32 + lane) * 4));
+    if (lane == 0)
+        *scale_out = scale;
+    __syncwarp();  // the stage has been read
+}
+
+// One warp per (unit, KV head), K and V; a unit is one page of one sequence that
 // the call touches.  Sequence b owns the units from cu[b] / 16 + 2 b on: n new
-// tokens behind any remainder touch at most n / 16 + 2 pages, so the ranges
-// are disjoint and a unit finds its sequence by a binary search of cu, without
-// a scan over the batch.  Lane i holds dimensions 4 i .. 4 i + 3 of all 16
-// tokens, so a tile is read once, in whole rows, and the maximum, the codes
-// and the 4 x 4 byte transposes of V stay in registers.  The sequence's first
-// unit alone reads and writes its tail, each lane the dimensions that it owns:
-// the old tokens are in registers before the new ones are stored.
+// tokens behind any remainder touch at most n / 16 + 2 pages, so the ranges are
+// disjoint and a unit finds its sequence by a search of cu, 32 ways at a time,
+// without a scan over the batch.  Lane i holds dimensions 4 i .. 4 i + 3 of all 16
+// tokens of both planes, so they are read once, in whole rows, with 8 KiB a warp
+// under way, and the maximum, the codes and the 4 x 4 byte transposes of V stay in
+// registers.  The sequence's first unit alone reads and writes its tail, each lane
+// the dimensions that it owns: the old tokens are in registers before the new ones
+// are stored.
 template <uint32_t FMT, bool F32>
-__global__ void __launch_bounds__(kAppendWarps * 32) kv8_append_kernel(const AppendArgs a)
+__global__ void __launch_bounds__(kAppendWarps * 32, 2) kv8_append_kernel(const AppendArgs a)
 {
     __shared__ __align__(16) uint32_t stage[kAppendWarps][kPlane / 4];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -95,25 +182,25 @@ __global__ void __launch_bounds__(kAppendWarps * 32) kv8_append_kernel(const App
                              (uint32_t)a.cu[gid + 1] > a.num_tokens))
         flag_error(a.error, kErrCu);
     const uint64_t item = gid >> 5;
-    if (item >= a.n_warps)
+    if (item >= a.n_items)
         return;
-    const uint32_t plane = (uint32_t)(item & 1u);
-    const uint32_t h = (uint32_t)((item >> 1) % a.num_kv_heads);
-    const int64_t unit = (int64_t)((item >> 1) / a.num_kv_heads);
+    const uint32_t h = (uint32_t)(item % a.num_kv_heads);
+    const int64_t unit = (int64_t)(item / a.num_kv_heads);
 
-    uint32_t lo = 0, hi = a.num_seqs;  // the last b with cu[b] / 16 + 2 b <= unit
-    while (hi - lo > 1u) {
-        const uint32_t mid = (lo + hi) >> 1;
-        if ((int64_t)(a.cu[mid] >> 4) + 2 * (int64_t)mid <= unit)
-            lo = mid;
-        else
-            hi = mid;
+    // the last b with cu[b] / 16 + 2 b <= unit, or 0
+    uint32_t b = 0, n = a.num_seqs;
+    while (n > 1) {
+        const uint32_t step = (n + 31) / 32, at = b + step * (uint32_t)lane;
+        const bool before = step * (uint32_t)lane < n && (int64_t)(a.cu[at] >> 4) + 2 * (int64_t)at <= unit;
+        // cu may decrease in a bad call: then any b will do
+        const int last = 31 - __clz(__ballot_sync(0xFFFFFFFFu, before) | 1u);
+        n = min(step, n - step * (uint32_t)last);
+        b += step * (uint32_t)last;
     }
-    const uint32_t b = lo;
-    const int64_t c0 = a.cu[b], c1 = a.cu[b + 1], j = unit - ((c0 >> 4) + 2 * (int64_t)b);
+    const int64_t c0 = a.cu[b], c1 = a.cu[b + 1], L0 = a.lens[b], j = unit - ((c0 >> 4) + 2 * (int64_t)b);
     if (j < 0 || c0 < 0 || c1 <= c0 || c1 > (int64_t)a.num_tokens)
         return;
-    const int64_t L0 = a.lens[b], L1 = L0 + (c1 - c0);
+    const int64_t L1 = L0 + (c1 - c0);
     if (L0 < 0 || (L1 >> 4) > (int64_t)a.max_pages) {
         if (lane == 0)
             flag_error(a.error, kErrLen);
@@ -123,72 +210,53 @@ __global__ void __launch_bounds__(kAppendWarps * 32) kv8_append_kernel(const App
     const bool full = first + 16 <= L1;
     if (!full && j > 0)
         return;
-    const void *src = plane ? a.v : a.k;
-    const uint64_t stride = plane ? a.v_stride : a.k_stride;
     const uint64_t col = (uint64_t)h * 128u + 4u * lane;
-    __nv_bfloat16 *tail = a.tail + rt_page_elem_offset(b, h, plane, 0, a.num_kv_heads) + 4 * lane;
+    __nv_bfloat16 *tail = a.tail + rt_page_elem_offset(b, h, 0, 0, a.num_kv_heads) + 4 * lane;
 
     if (full) {
-        uint2 x[16];
+        const int32_t id = a.page_table[(uint64_t)b * a.max_pages + page];
+        uint2 x[2][16];
+        if (first >= L0) {  // new tokens alone
+            const uint64_t row = (uint64_t)(c0 + first - L0);
+            uint64_t at_k = row * a.k_stride + col, at_v = row * a.v_stride + col;
 #pragma unroll
-        for (int t = 0; t < 16; t++) {
-            const int64_t pos = first + t;
-            x[t] = pos < L0 ? *reinterpret_cast<const uint2 *>(tail + t * 128)
-                            : load4<F32>(src, (uint64_t)(c0 + pos - L0) * stride + col);
+            for (int t = 0; t < 16; t++) {
+                x[0][t] = load4<F32>(a.k, at_k);
+                x[1][t] = load4<F32>(a.v, at_v);
+                at_k += a.k_stride;
+                at_v += a.v_stride;
+            }
+        } else {
+#pragma unroll
+            for (int t = 0; t < 16; t++) {
+                const int64_t pos = first + t;
+                if (pos < L0) {
+                    x[0][t] = *reinterpret_cast<const uint2 *>(tail + t * 128);
+                    x[1][t] = *reinterpret_cast<const uint2 *>(tail + 2048 + t * 128);
+                } else {
+                    const uint64_t row = (uint64_t)(c0 + pos - L0);
+                    x[0][t] = load4<F32>(a.k, row * a.k_stride + col);
+                    x[1][t] = load4<F32>(a.v, row * a.v_stride + col);
+                }
+            }
         }
-        uint32_t top2 = 0;  // per 16-bit half: the largest magnitude's bits
-#pragma unroll
-        for (int t = 0; t < 16; t++)
-            top2 = __vmaxu2(top2, __vmaxu2(x[t].x & 0x7FFF7FFFu, x[t].y & 0x7FFF7FFFu));
-        const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, max(top2 & 0xFFFFu, top2 >> 16));
-        // a NaN's or infinity's bits are above every number's
-        const float scale = top >= 0x7F80u ? __int_as_float(0x7FC00000)
-                                           : __fdiv_rn(__uint_as_float(top << 16),
-                                                       FMT == RT_KV8_E4M3 ? 448.0f : 127.0f);
-        uint32_t w[16];
-#pragma unroll
-        for (int t = 0; t < 16; t++)
-            w[t] = scale > 0.0f ? quantise4<FMT>(x[t], scale) : 0u;
-        const int32_t id = a.page_table[(size_t)b * a.max_pages + page];
         if (id < 0 || (uint64_t)id >= a.arena_pages) {
             if (lane == 0)
                 flag_error(a.error, kErrPage);
         } else {
-            uint32_t *s = stage[warp];
-            if (plane == 0) {
-#pragma unroll
-                for (int t = 0; t < 16; t++)
-                    s[rt_kv8_k_offset(t, 4 * lane) / 4] = w[t];
-            } else {
-                // words of tokens {2c, 2c+1, 2c+8, 2c+9} x 4 dimensions -> 4 words of 4 tokens
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    const uint32_t r0 = w[2 * c], r1 = w[2 * c + 1], r2 = w[2 * c + 8],
-                                   r3 = w[2 * c + 9];
-                    const uint32_t p0 = __byte_perm(r0, r1, 0x5140), p1 = __byte_perm(r0, r1, 0x7362);
-                    const uint32_t q0 = __byte_perm(r2, r3, 0x5140), q1 = __byte_perm(r2, r3, 0x7362);
-                    const uint32_t o[4] = {__byte_perm(p0, q0, 0x5410), __byte_perm(p0, q0, 0x7632),
-                                           __byte_perm(p1, q1, 0x5410), __byte_perm(p1, q1, 0x7632)};
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        s[rt_kv8_v_offset(2 * c, 4 * lane + e) / 4] = o[e];
-                }
-            }
-            __syncwarp();
-            const uint64_t tile = ((uint64_t)id * a.num_kv_heads + h) * 2u + plane;
-            uint4 *dst = reinterpret_cast<uint4 *>(a.pages + tile * kPlane);
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                dst[i * 32 + lane] = reinterpret_cast<const uint4 *>(s)[i * 32 + lane];
-            if (lane == 0)
-                a.scales[tile] = scale;
+            const uint64_t tile = ((uint64_t)id * a.num_kv_heads + h) * 2u;
+            store_tile<FMT>(x[0], 0, stage[warp], a.pages + tile * kPlane, a.scales + tile);
+            store_tile<FMT>(x[1], 1, stage[warp], a.pages + (tile + 1) * kPlane, a.scales + tile + 1);
         }
     }
     if (j == 0) {
         const int64_t base = (L1 >> 4) << 4;
-        for (int64_t pos = base > L0 ? base : L0; pos < L1; pos++)
-            *reinterpret_cast<uint2 *>(tail + (pos - base) * 128) =
-                load4<F32>(src, (uint64_t)(c0 + pos - L0) * stride + col);
+        for (int64_t pos = base > L0 ? base : L0; pos < L1; pos++) {
+            const uint64_t row = (uint64_t)(c0 + pos - L0);
+            __nv_bfloat16 *to = tail + (pos - base) * 128;
+            *reinterpret_cast<uint2 *>(to) = load4<F32>(a.k, row * a.k_stride + col);
+            *reinterpret_cast<uint2 *>(to + 2048) = load4<F32>(a.v, row * a.v_stride + col);
+        }
     }
 }
 
@@ -1073,8 +1141,8 @@ extern "C" int rt_kv8_append(const rt_kv8_append_params_t *p, const void *k, con
     a.num_tokens = p->num_tokens;
     a.max_pages = p->max_pages_per_seq;
     const uint64_t units = (uint64_t)p->num_tokens / 16u + 2ull * p->num_seqs;
-    a.n_warps = units * p->num_kv_heads * 2u;
-    const uint64_t blocks = (a.n_warps + kAppendWarps - 1) / kAppendWarps;
+    a.n_items = units * p->num_kv_heads;
+    const uint64_t blocks = (a.n_items + kAppendWarps - 1) / kAppendWarps;
     if (blocks > 0x7FFFFFFFull) {
         rt::set_error("kv8_append: more than 2^31 - 1 blocks of work; append in parts");
         return RT_EINVAL;

@@ -135,39 +135,12 @@ __device__ __forceinline__ T from_float(float x)
         return x;
 }
 
-// Two fp32 values in one register pair: sm_100 adds, multiplies and fuses them in
-// one instruction each.
-typedef uint64_t f32x2;
-__device__ __forceinline__ f32x2 pair(float lo, float hi)
-{
-    f32x2 r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-    return r;
-}
-__device__ __forceinline__ float2 halves(f32x2 v)
-{
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
-}
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c)
-{
-    f32x2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b)
-{
-    f32x2 r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b)
-{
-    f32x2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
+using rt::f32x2;
+using rt::pair;
+using rt::halves;
+using rt::fma2;
+using rt::add2;
+using rt::mul2;
 __device__ __forceinline__ f32x2 exp2_2(f32x2 z)
 {
     const float2 v = halves(z);
