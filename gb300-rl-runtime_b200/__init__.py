@@ -8,7 +8,6 @@ fails loudly if the shared library has not been built - there is no fallback.
 """
 from __future__ import annotations
 
-import collections
 import contextlib
 import ctypes
 import os
@@ -473,54 +472,70 @@ def _need(ok, what):
 def _same_device(first, *others):
     """Every tensor given lies on the first one's CUDA device."""
     dev = first.device
-    _need(dev.type == "cuda", "tensors must be on a CUDA device")
+    if dev.type != "cuda":
+        raise ValueError("tensors must be on a CUDA device")
     for t in others:
-        _need(t is None or t.device == dev, "tensors must be on one device")
+        if t is not None and t.device != dev:
+            raise ValueError("tensors must be on one device")
     return dev
 
 
 _HERE = contextlib.nullcontext()
+_torch = None
+_DTYPES = {}
+_KV8_FORMATS = {}
+
+
+def _tm():
+    """torch, imported at the first call that needs it."""
+    global _torch
+    if _torch is None:
+        import torch
+        _DTYPES.update({torch.float32: RT_DTYPE_F32, torch.bfloat16: RT_DTYPE_BF16})
+        _KV8_FORMATS.update({torch.float8_e4m3fn: RT_KV8_E4M3, torch.int8: RT_KV8_S8})
+        _torch = torch
+    return _torch
 
 
 def _on(dev, stream):
     """A context in which the tensors' device is current, and `stream` where one is given (so
     that what is allocated inside belongs to the stream that uses it), and the stream's handle."""
-    import torch
+    torch = _torch
     if stream is not None:
         _need(stream.device == dev, "the stream is another device's")
         return torch.cuda.stream(stream), stream.cuda_stream
-    s = torch.cuda.current_stream(dev).cuda_stream
-    return (_HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)), s
+    if torch.cuda.current_device() == dev.index:
+        return _HERE, torch._C._cuda_getCurrentRawStream(dev.index)
+    return torch.cuda.device(dev), torch.cuda.current_stream(dev).cuda_stream
 
 
 def _error_word(error):
-    import torch
     if error is None:
         return None
-    _need(error.dtype == torch.int32 and error.numel() == 1, "error: one int32")
+    _need(error.dtype == _torch.int32 and error.numel() == 1, "error: one int32")
     return error.data_ptr()
 
 
 def _int_array(t, shape, what):
-    import torch
-    _need(t.dtype == torch.int32 and t.shape == shape and t.is_contiguous(),
-          f"{what}: contiguous int32 {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    if t.dtype != _torch.int32 or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{what}: contiguous int32 {tuple(shape)}, got {t.dtype} "
+                         f"{tuple(t.shape)}")
     return t.data_ptr()
 
 
 def _kv8_cache(pages, scales, tail, num_seqs):
-    """(format, KV heads) of a cache's buffers, checked."""
-    import torch
-    fmt = {torch.float8_e4m3fn: RT_KV8_E4M3, torch.int8: RT_KV8_S8}.get(pages.dtype)
-    _need(fmt is not None, f"pages: float8_e4m3fn or int8, got {pages.dtype}")
-    _need(pages.dim() == 4 and tuple(pages.shape[2:]) == (2, KV8_PLANE_BYTES)
-          and pages.is_contiguous(), "pages: contiguous [n, kv heads, 2, 2048]")
-    n, h = pages.shape[:2]
+    """(format, pages, KV heads) of a cache's buffers, checked."""
+    torch = _torch
+    fmt = _KV8_FORMATS.get(pages.dtype)
+    _need(fmt is not None, "pages: float8_e4m3fn or int8")
+    _need(pages.dim() == 4 and pages.is_contiguous(), "pages: contiguous [n, kv heads, 2, 2048]")
+    n, h, planes, size = pages.shape
+    _need(planes == 2 and size == KV8_PLANE_BYTES, "pages: contiguous [n, kv heads, 2, 2048]")
     _need(scales.dtype == torch.float32 and scales.shape == (n, h, 2) and scales.is_contiguous(),
           "scales: contiguous float32 [n, kv heads, 2]")
     _need(tail.dtype == torch.bfloat16 and tail.shape == (num_seqs, h, 2, 16, 128)
           and tail.is_contiguous(), "tail: contiguous bfloat16 [sequences, kv heads, 2, 16, 128]")
-    return fmt, h
+    return fmt, n, h
 
 
 def kv8_cache(n_pages, num_seqs, num_kv_heads, format="e4m3", device="cuda"):
@@ -540,24 +555,27 @@ def kv8_append(k, v, cu_tokens, seq_lens, page_table, pages, scales, tail, error
     [T, kv heads, 128], any token stride that is a multiple of 8) behind the seq_lens[b]
     tokens that sequence b has.  cu_tokens int32 [B + 1], seq_lens int32 [B], page_table
     int32 [B, P]; pages, scales and tail as kv8_cache makes them.  seq_lens is not advanced."""
-    import torch
+    _tm()
     B = seq_lens.shape[0]
     dev = _same_device(pages, k, v, cu_tokens, seq_lens, page_table, scales, tail, error)
-    fmt, h = _kv8_cache(pages, scales, tail, B)
-    dtype = {torch.float32: RT_DTYPE_F32, torch.bfloat16: RT_DTYPE_BF16}.get(k.dtype)
+    fmt, n_pages, h = _kv8_cache(pages, scales, tail, B)
+    dtype = _DTYPES.get(k.dtype)
     _need(dtype is not None and v.dtype == k.dtype, "k, v: both bfloat16 or both float32")
     T = k.shape[0]
-    for t in (k, v):
-        _need(t.shape == (T, h, 128) and t.stride(2) == 1 and (h == 1 or t.stride(1) == 128),
-              "k, v: [tokens, kv heads, 128] with contiguous heads")
+    shape, row = (T, h, 128), h * 128
+    k_stride, k_head, k_dim = k.stride() if k.shape == shape else (0, 0, 0)
+    v_stride, v_head, v_dim = v.stride() if v.shape == shape else (0, 0, 0)
+    _need(k_dim == 1 and v_dim == 1 and (h == 1 or (k_head == 128 and v_head == 128)),
+          "k, v: [tokens, kv heads, 128] with contiguous heads")
     _need(page_table.dim() == 2 and page_table.shape[0] == B, "page_table: int32 [sequences, P]")
-    strides = [t.stride(0) if T > 1 else h * 128 for t in (k, v)]
-    p = rt_kv8_append_params_t(B, h, T, page_table.shape[1], pages.shape[0], *strides, fmt, dtype)
-    args = (_int_array(cu_tokens, (B + 1,), "cu_tokens"), _int_array(seq_lens, (B,), "seq_lens"),
-            _int_array(page_table, page_table.shape, "page_table"))
+    P = page_table.shape[1]
+    p = rt_kv8_append_params_t(B, h, T, P, n_pages, k_stride if T > 1 else row,
+                               v_stride if T > 1 else row, fmt, dtype)
+    cu, lens = _int_array(cu_tokens, (B + 1,), "cu_tokens"), _int_array(seq_lens, (B,), "seq_lens")
+    table = _int_array(page_table, (B, P), "page_table")
     ctx, s = _on(dev, stream)
     with ctx:
-        check(lib().rt_kv8_append(ctypes.byref(p), k.data_ptr(), v.data_ptr(), *args,
+        check(lib().rt_kv8_append(ctypes.byref(p), k.data_ptr(), v.data_ptr(), cu, lens, table,
                                   pages.data_ptr(), scales.data_ptr(), tail.data_ptr(),
                                   _error_word(error), s), "rt_kv8_append")
 
@@ -567,36 +585,39 @@ def kv8_decode_attention(q, pages, scales, tail, page_table, seq_lens, max_seq_l
     """rt_kv8_decode_attention: q bf16 [B, Hq, 128] over the cache of kv8_append; returns
     fp32 [B, Hq, 128].  max_seq_len bounds every seq_lens[b].  workspace: uint8, by default
     a new one (from torch's allocator, on the current stream)."""
-    import torch
+    torch = _tm()
     B = seq_lens.shape[0]
     dev = _same_device(q, pages, scales, tail, page_table, seq_lens, out, workspace, error)
-    fmt, h = _kv8_cache(pages, scales, tail, B)
-    _need(q.dtype == torch.bfloat16 and q.dim() == 3 and q.shape[0] == B and q.shape[2] == 128
-          and q.stride(2) == 1 and (q.shape[1] == 1 or q.stride(1) == 128),
+    fmt, n_pages, h = _kv8_cache(pages, scales, tail, B)
+    _need(q.dtype == torch.bfloat16 and q.dim() == 3, "q: bfloat16 [sequences, heads, 128]")
+    n, Hq, dim = q.shape
+    q_stride, q_head, q_dim = q.stride()
+    _need(n == B and dim == 128 and q_dim == 1 and (Hq == 1 or q_head == 128),
           "q: bfloat16 [sequences, heads, 128] with contiguous heads")
-    Hq = q.shape[1]
     _need(out is None or (out.dtype == torch.float32 and out.shape == (B, Hq, 128)
                           and out.is_contiguous()),
           "out: contiguous float32 [sequences, heads, 128]")
     _need(page_table.dim() == 2 and page_table.shape[0] == B, "page_table: int32 [sequences, P]")
+    P = page_table.shape[1]
     _need(0 <= max_seq_len <= 0x7FFFFFFF and 0 <= chunk_pages <= 128,
           "max_seq_len 0 .. 2^31 - 1, chunk_pages 0 .. 128")
-    p = rt_kv8_attn_params_t(B, Hq, h, page_table.shape[1], max_seq_len, fmt, pages.shape[0],
-                             q.stride(0) if B > 1 else Hq * 128,
-                             scale if scale is not None else 128 ** -0.5, chunk_pages)
-    args = (_int_array(page_table, page_table.shape, "page_table"),
-            _int_array(seq_lens, (B,), "seq_lens"))
+    p = rt_kv8_attn_params_t(B, Hq, h, P, max_seq_len, fmt, n_pages,
+                             q_stride if B > 1 else Hq * 128,
+                             128 ** -0.5 if scale is None else scale, chunk_pages)
+    ref = ctypes.byref(p)
+    table, lens = _int_array(page_table, (B, P), "page_table"), _int_array(seq_lens, (B,), "seq_lens")
     ctx, s = _on(dev, stream)
     with ctx:
         if out is None:
-            out = torch.empty(B, Hq, 128, dtype=torch.float32, device=dev)
-        need = lib().rt_kv8_attn_workspace_bytes(ctypes.byref(p))
-        if need and workspace is None:
-            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+            out = torch.empty((B, Hq, 128), dtype=torch.float32, device=dev)
+        size = lib().rt_kv8_attn_workspace_bytes(ref)
+        if size and workspace is None:
+            workspace = torch.empty(size, dtype=torch.uint8, device=dev)
+        elif workspace is not None:
+            size = workspace.numel() * workspace.element_size()
         check(lib().rt_kv8_decode_attention(
-            ctypes.byref(p), q.data_ptr(), pages.data_ptr(), scales.data_ptr(), tail.data_ptr(),
-            *args, out.data_ptr(), None if workspace is None else workspace.data_ptr(),
-            0 if workspace is None else workspace.numel() * workspace.element_size(),
+            ref, q.data_ptr(), pages.data_ptr(), scales.data_ptr(), tail.data_ptr(), table, lens,
+            out.data_ptr(), None if workspace is None else workspace.data_ptr(), size,
             _error_word(error), s), "rt_kv8_decode_attention")
     return out
 
@@ -1078,41 +1099,35 @@ def grpo_advantages(rewards, group, eps=1e-6, out=None, stream=None):
 
 def _rows_of(logits, tokens):
     """(rows, vocab, row stride, dtype) of a matrix of logits and its tokens, checked."""
-    import torch
-    dtype = {torch.float32: RT_DTYPE_F32, torch.bfloat16: RT_DTYPE_BF16}.get(logits.dtype)
+    dtype = _DTYPES.get(logits.dtype)
     _need(dtype is not None and logits.dim() == 2, "logits: bfloat16 or float32 [rows, vocab]")
     R, V = logits.shape
-    _need(V == 1 or logits.stride(1) == 1, "logits: contiguous rows")
-    _need(tokens.dtype in (torch.int32, torch.uint32) and tokens.shape == (R,)
-          and tokens.is_contiguous(), "tokens: contiguous int32 [rows]")
-    return R, V, (logits.stride(0) if R > 1 else V), dtype
+    stride, step = logits.stride()
+    _need(V == 1 or step == 1, "logits: contiguous rows")
+    return R, V, (stride if R > 1 else V), dtype, _index_array(tokens, R, "tokens")
 
 
 def _float_array(t, n, what):
-    import torch
     if t is None:
         return None
-    _need(t.dtype == torch.float32 and t.shape == (n,) and t.is_contiguous(),
-          f"{what}: contiguous float32 [{n}], got {t.dtype} {tuple(t.shape)}")
+    if t.dtype != _torch.float32 or t.shape != (n,) or not t.is_contiguous():
+        raise ValueError(f"{what}: contiguous float32 [{n}], got {t.dtype} {tuple(t.shape)}")
     return t.data_ptr()
 
 
 def _index_array(t, n, what):
-    import torch
     if t is None:
         return None
-    _need(t.dtype in (torch.int32, torch.uint32) and t.shape == (n,) and t.is_contiguous(),
-          f"{what}: contiguous int32 [{n}]")
+    if t.dtype not in (_torch.int32, _torch.uint32) or t.shape != (n,) or not t.is_contiguous():
+        raise ValueError(f"{what}: contiguous int32 [{n}], got {t.dtype} {tuple(t.shape)}")
     return t.data_ptr()
 
 
-def _gradient_of(logits, dlogits):
+def _gradient_of(logits, dlogits, R, V):
     """The gradient's buffer (a new one for None) and its row stride."""
-    import torch
-    R, V = logits.shape
     if dlogits is None:
-        dlogits = torch.empty(R, V, dtype=logits.dtype, device=logits.device)
-    _need(dlogits.dtype == logits.dtype and dlogits.shape == logits.shape
+        return _torch.empty((R, V), dtype=logits.dtype, device=logits.device), V
+    _need(dlogits.dtype == logits.dtype and dlogits.shape == (R, V)
           and (V == 1 or dlogits.stride(1) == 1), "dlogits: the logits' type and shape")
     return dlogits, (dlogits.stride(0) if R > 1 else V)
 
@@ -1122,8 +1137,8 @@ def token_logprobs(logits, tokens, temperature=1.0, row_enable=None, logprobs=No
     """rt_token_logprobs: (log-probability of each row's token, entropy of each row), fp32 [R],
     of logits fp32 or bf16 [R, V] (any row stride) and tokens int32 [R].  Rows whose row_enable
     (int32 [R]) is 0 are skipped: give logprobs and entropy to know what they hold."""
-    import torch
-    R, V, stride, dtype = _rows_of(logits, tokens)
+    torch = _tm()
+    R, V, stride, dtype, tok = _rows_of(logits, tokens)
     dev = _same_device(logits, tokens, row_enable, logprobs, entropy, error)
     p = rt_logprob_params_t(R, V, stride, 0, dtype, temperature,
                             _index_array(row_enable, R, "row_enable"))
@@ -1131,11 +1146,14 @@ def token_logprobs(logits, tokens, temperature=1.0, row_enable=None, logprobs=No
     with ctx:
         if logprobs is None:
             logprobs = torch.empty(R, dtype=torch.float32, device=dev)
+        else:
+            _float_array(logprobs, R, "logprobs")
         if entropy is None:
             entropy = torch.empty(R, dtype=torch.float32, device=dev)
-        check(lib().rt_token_logprobs(ctypes.byref(p), logits.data_ptr(), tokens.data_ptr(),
-                                      _float_array(logprobs, R, "logprobs"),
-                                      _float_array(entropy, R, "entropy"), _error_word(error), s),
+        else:
+            _float_array(entropy, R, "entropy")
+        check(lib().rt_token_logprobs(ctypes.byref(p), logits.data_ptr(), tok, logprobs.data_ptr(),
+                                      entropy.data_ptr(), _error_word(error), s),
               "rt_token_logprobs")
     return logprobs, entropy
 
@@ -1144,24 +1162,38 @@ def token_logprobs_backward(logits, tokens, dlogprobs, dentropy=None, temperatur
                             row_enable=None, dlogits=None, error=None, stream=None):
     """rt_token_logprobs_backward: the gradient with respect to the logits, in their type;
     dlogits may be the logits themselves."""
-    R, V, stride, dtype = _rows_of(logits, tokens)
+    _tm()
+    R, V, stride, dtype, tok = _rows_of(logits, tokens)
     dev = _same_device(logits, tokens, dlogprobs, dentropy, row_enable, dlogits, error)
     ctx, s = _on(dev, stream)
     with ctx:
-        dlogits, grad_stride = _gradient_of(logits, dlogits)
+        dlogits, grad_stride = _gradient_of(logits, dlogits, R, V)
         p = rt_logprob_params_t(R, V, stride, grad_stride, dtype, temperature,
                                 _index_array(row_enable, R, "row_enable"))
         check(lib().rt_token_logprobs_backward(
-            ctypes.byref(p), logits.data_ptr(), tokens.data_ptr(),
-            _float_array(dlogprobs, R, "dlogprobs"), _float_array(dentropy, R, "dentropy"),
-            dlogits.data_ptr(), _error_word(error), s), "rt_token_logprobs_backward")
+            ctypes.byref(p), logits.data_ptr(), tok, _float_array(dlogprobs, R, "dlogprobs"),
+            _float_array(dentropy, R, "dentropy"), dlogits.data_ptr(), _error_word(error), s),
+            "rt_token_logprobs_backward")
     return dlogits
 
 
-# stats fp32 [5]: weighted sums of loss, policy, kl, entropy, clipped; then fp32 [R] columns of
-# the rows' records (rt_policy_row_t) and the gradient (None when not asked for)
-PolicyLoss = collections.namedtuple(
-    "PolicyLoss", "stats logprobs entropy row_loss policy kl ratio clipped dlogits")
+class PolicyLoss:
+    """What policy_loss computed: stats fp32 [5] (the rows' sums of weight times loss, policy, kl,
+    entropy, clipped), dlogits (None when not asked for), rows fp32 [R, 8] (rt_policy_row_t) and
+    its columns as fp32 [R]: logprobs, entropy, row_loss, policy, kl, ratio, clipped."""
+
+    __slots__ = ("stats", "rows", "dlogits")
+
+    def __init__(self, stats, rows, dlogits):
+        self.stats, self.rows, self.dlogits = stats, rows, dlogits
+
+    logprobs = property(lambda self: self.rows[:, 0])
+    entropy = property(lambda self: self.rows[:, 1])
+    row_loss = property(lambda self: self.rows[:, 2])
+    policy = property(lambda self: self.rows[:, 3])
+    kl = property(lambda self: self.rows[:, 4])
+    ratio = property(lambda self: self.rows[:, 5])
+    clipped = property(lambda self: self.rows[:, 6])
 
 
 def policy_loss(logits, tokens, weights, advantages, old_logprobs=None, ref_logprobs=None,
@@ -1171,32 +1203,31 @@ def policy_loss(logits, tokens, weights, advantages, old_logprobs=None, ref_logp
     gradient.  weights fp32 [R]; advantages fp32 [S], one per rollout, with row_seq int32 [R]
     naming each row's (None: one per row); old_logprobs None: on-policy.  dlogits may be the
     logits themselves; backward=False computes the values alone.  Returns a PolicyLoss."""
-    import torch
-    R, V, stride, dtype = _rows_of(logits, tokens)
+    torch = _tm()
+    R, V, stride, dtype, tok = _rows_of(logits, tokens)
     dev = _same_device(logits, tokens, weights, advantages, old_logprobs, ref_logprobs, row_seq,
                        dlogits, error)
     _need(backward or dlogits is None, "dlogits without backward")
     _need(advantages.dim() == 1 and (row_seq is not None or advantages.shape[0] == R),
           "advantages: one per row without row_seq")
+    S = advantages.shape[0]
     ctx, s = _on(dev, stream)
     with ctx:
         grad_stride = 0
         if backward:
-            dlogits, grad_stride = _gradient_of(logits, dlogits)
-        rows = torch.empty(R, 8, dtype=torch.float32, device=dev)
+            dlogits, grad_stride = _gradient_of(logits, dlogits, R, V)
+        rows = torch.empty((R, 8), dtype=torch.float32, device=dev)
         stats = torch.empty(5, dtype=torch.float32, device=dev)
-        p = rt_policy_params_t(R, V, advantages.shape[0], dtype, stride, grad_stride, temperature,
-                               clip_low, clip_high, kl_coef, entropy_coef)
+        p = rt_policy_params_t(R, V, S, dtype, stride, grad_stride, temperature, clip_low,
+                               clip_high, kl_coef, entropy_coef)
         check(lib().rt_policy_loss(
-            ctypes.byref(p), logits.data_ptr(), tokens.data_ptr(),
-            _float_array(weights, R, "weights"),
-            _float_array(advantages, advantages.shape[0], "advantages"),
-            _index_array(row_seq, R, "row_seq"), _float_array(old_logprobs, R, "old_logprobs"),
+            ctypes.byref(p), logits.data_ptr(), tok, _float_array(weights, R, "weights"),
+            _float_array(advantages, S, "advantages"), _index_array(row_seq, R, "row_seq"),
+            _float_array(old_logprobs, R, "old_logprobs"),
             _float_array(ref_logprobs, R, "ref_logprobs"), rows.data_ptr(), stats.data_ptr(),
             None if dlogits is None else dlogits.data_ptr(), _error_word(error), s),
             "rt_policy_loss")
-    c = rows.unbind(1)
-    return PolicyLoss(stats, c[0], c[1], c[2], c[3], c[4], c[5], c[6], dlogits)
+    return PolicyLoss(stats, rows, dlogits)
 
 
 class NcclRewards:

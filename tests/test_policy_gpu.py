@@ -341,8 +341,7 @@ def test_policy_of_padded_rows(pkg, cuda):
     d = torch.full((30, 2003), 3.0, dtype=torch.bfloat16, device=cuda)
     r = pkg.policy_loss(**c, kl_coef=0.04, entropy_coef=0.01, error=error, dlogits=d)
     assert error.item() == 0
-    for col in r[1:8]:
-        assert bool((col[::3] == 0).all())
+    assert bool((r.rows[::3] == 0).all())
     assert bool((r.dlogits[::3] == 0).all()) and bool(torch.isfinite(r.stats).all())
     c["tokens"][0], c["row_seq"][3] = 0, 0
     c["old_logprobs"][::3] = 0.0
@@ -375,8 +374,8 @@ def test_policy_gradient_in_place_and_again(pkg, cuda):
     c = case(cuda, 50, 32000, torch.float32, 23)
     first = pkg.policy_loss(**c, kl_coef=0.04, entropy_coef=0.01)
     again = pkg.policy_loss(**c, kl_coef=0.04, entropy_coef=0.01)
-    for x, y in zip(first, again):
-        assert torch.equal(x, y)                              # the same bits every time
+    for name in ("stats", "rows", "dlogits"):                 # the same bits every time
+        assert torch.equal(getattr(first, name), getattr(again, name))
     same = pkg.policy_loss(**c, kl_coef=0.04, entropy_coef=0.01, dlogits=c["logits"])
     assert same.dlogits.data_ptr() == c["logits"].data_ptr()
     assert torch.equal(same.dlogits, first.dlogits) and torch.equal(same.stats, first.stats)
@@ -425,8 +424,8 @@ def test_policy_captured_and_replayed(pkg, cuda):
         graph.replay()
         torch.cuda.synchronize()
         want = pkg.policy_loss(**new, **kw)
-        for x, y in zip(r, want):
-            assert torch.equal(x, y)
+        for name in ("stats", "rows", "dlogits"):
+            assert torch.equal(getattr(r, name), getattr(want, name))
 
 
 def test_rows_beyond_32_bits(pkg, cuda):
