@@ -1187,13 +1187,13 @@ class PolicyLoss:
     def __init__(self, stats, rows, dlogits):
         self.stats, self.rows, self.dlogits = stats, rows, dlogits
 
-    logprobs = property(lambda self: self.rows[:, 0])
-    entropy = property(lambda self: self.rows[:, 1])
-    row_loss = property(lambda self: self.rows[:, 2])
-    policy = property(lambda self: self.rows[:, 3])
-    kl = property(lambda self: self.rows[:, 4])
-    ratio = property(lambda self: self.rows[:, 5])
-    clipped = property(lambda self: self.rows[:, 6])
+    logprobs = property(lambda self: self.rows.select(1, 0))
+    entropy = property(lambda self: self.rows.select(1, 1))
+    row_loss = property(lambda self: self.rows.select(1, 2))
+    policy = property(lambda self: self.rows.select(1, 3))
+    kl = property(lambda self: self.rows.select(1, 4))
+    ratio = property(lambda self: self.rows.select(1, 5))
+    clipped = property(lambda self: self.rows.select(1, 6))
 
 
 def policy_loss(logits, tokens, weights, advantages, old_logprobs=None, ref_logprobs=None,

@@ -1134,7 +1134,12 @@ __global__ void __launch_bounds__(WARPS == 1 ? 256 : WARPS * 32) kv8_merge_kerne
     }
 }
 
-// Pages per item.
+// Pages per item.  Where all rows' pages make two items to an SM of up to 128 pages
+// each, so many: fewer leave bandwidth idle, more are merged longer (1 x 131,071
+// tokens, 4 KV heads: 28 us, with 48 pages an item 34, 32: 38).  Larger batches have
+// more items than fit at once, and an item's start and end cost about as much as 14
+// pages: 96 pages (64 sequences of up to 4,096: 58 us, with 32 pages 65; 16 of up to
+// 8,192: 34 against 40).
 struct AttnPlan {
     uint32_t chunk_pages, max_chunks;
     size_t part_o, part_ml;
@@ -1144,11 +1149,11 @@ AttnPlan plan_of(const rt_kv8_attn_params_t *p)
 {
     AttnPlan r;
     const uint64_t rows = (uint64_t)p->num_seqs * p->num_kv_heads, pages = p->max_seq_len >> 4;
-    const uint64_t items = 3ull * kCtasPerSm * (uint64_t)rt::num_sms();
     uint64_t c = p->chunk_pages;
     if (!c) {
-        c = (pages * rows + items - 1) / items;
-        c = c < 32 ? 32 : c > kMaxChunkPages ? kMaxChunkPages : c;
+        const uint64_t per_row = rows ? 2ull * (uint64_t)rt::num_sms() / rows : 1u;
+        c = per_row ? (pages + per_row - 1) / per_row : kMaxChunkPages + 1u;
+        c = c > kMaxChunkPages ? 96u : c < 16u ? 16u : c;
     }
     r.chunk_pages = (uint32_t)((c + 1) / 2 * 2);  // whole pairs
     r.max_chunks = (uint32_t)((pages + r.chunk_pages - 1) / r.chunk_pages);
