@@ -30,7 +30,7 @@ constexpr int kCtasPerSm = 4;
 constexpr int kRowWarps = 8;
 constexpr int kThreads = kRowWarps * 32;
 constexpr uint32_t kMaxCluster = 8;
-constexpr uint32_t kMaxRows = 32;  // of a cluster or warp, one to a lane
+constexpr uint32_t kMaxRows = 32;  // of a group, one to a lane
 constexpr uint32_t kMaxVocab = 262144;
 constexpr uint64_t kWaitLimitNs = 2000000000ull;
 constexpr uint32_t kSmemTarget = 72 * 1024;  // of a CTA: three to an SM
@@ -774,10 +774,12 @@ __global__ void __launch_bounds__(512) policy_stats_kernel(const rt_policy_row_t
 // Short rows, when there are enough of them for all SMs' warps, are a warp's own.
 // Else CTAs to a row: as few as make a slice fit the target, then more while the
 // rows would leave SMs idle and a slice keeps 8 KiB.  A group (a cluster or a warp)
-// takes several rows, so that the next row's copy starts as each warp ends its part
-// of the last: all groups at once where that makes a few rows each, so that no
-// group starts late; blocks of 8 where there are many, which the hardware balances
-// (8,192 rows of 32,000 fp32: 351 us, one row to a group 380).
+// that takes several rows starts each row's copy as its warps end their parts of the
+// row before.  Equal shares, all groups at once, where no group waits long for the
+// last (4,096 rows of 8,000 fp32, 6.9 turns: 50 us, one row to a group 62); else one
+// row to a group, balanced by the hardware (1,023 padded rows of 50,001 bf16, 3.5
+// turns: 46 us, shares of 4 51); blocks of 8 where there are many (8,192 rows of
+// 32,000 fp32: 345 us, one row to a group 380).
 template <typename T, Mode MODE, bool ALONE>
 int launch_rows(RowArgs &a, uint32_t k, cudaStream_t stream, const char *what)
 {
@@ -809,6 +811,8 @@ int launch_rows(RowArgs &a, uint32_t k, cudaStream_t stream, const char *what)
     uint64_t each = ((uint64_t)a.num_rows + at_once - 1) / at_once;
     if (!ALONE && each > 24)
         each = 8;
+    else if (!ALONE && each > 2 && a.num_rows * 100ull < each * at_once * 93u)
+        each = 1;
     a.rows_each = (uint32_t)(each > kMaxRows ? kMaxRows : each);
     const uint64_t in_groups = ((uint64_t)a.num_rows + a.rows_each - 1) / a.rows_each;
     const uint64_t ctas = (in_groups + groups - 1) / groups * k;
