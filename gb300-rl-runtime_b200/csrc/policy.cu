@@ -466,27 +466,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) row_kernel(const RowArgs
         // raised to there, which keeps 0 times -infinity out.
         Stats st{kNoRef, 0.0f, 0.0f};
         {
-            float limit = (float)(kNoRef + 64) * inv_c;
-            typename Eight<T>::Floor floor = Eight<T>::floor_of((float)(kNoRef - 200) * inv_c);
-            f32x2 minus_ref = pair(-(float)kNoRef, -(float)kNoRef), s2 = 0, u2 = 0;
             arrived(r);
-#pragma unroll 1
-            for (uint32_t v = r.lo + lane * N; v < r.hi; v += kStep) {
-                Eight<T> x;
-                x.load(here + (size_t)(v - r.lo) * sizeof(T), v + 32 * N < r.hi);
-                const float top = x.top();
-                if (top > limit) {  // a reference that is a little low does no harm
-                    const float2 s = halves(s2), u = halves(u2);
-                    st.s = s.x + s.y;
-                    st.u = u.x + u.y;
-                    raise(st, __float2int_rn(top * c));
-                    s2 = pair(st.s, 0.0f);
-                    u2 = pair(st.u, 0.0f);
-                    const float ref = (float)st.R;
-                    limit = (ref + 64.0f) * inv_c;
-                    floor = Eight<T>::floor_of((ref - 200.0f) * inv_c);
-                    minus_ref = pair(-ref, -ref);
-                }
+            const uint32_t bytes = (r.hi - r.lo) * (uint32_t)sizeof(T), mine = (uint32_t)lane * 16u;
+            f32x2 s2 = 0, u2 = 0, minus_ref;
+            auto add = [&](Eight<T> &x, typename Eight<T>::Floor floor) {
                 x.raise_to(floor);
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
@@ -494,14 +477,62 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) row_kernel(const RowArgs
                     s2 = add2(s2, e);
                     u2 = fma2(e, z, u2);
                 }
+            };
+            auto total = [&](f32x2 v) { return halves(v).x + halves(v).y; };
+            // The warp's first vectors give its reference.  It does not have to be the
+            // maximum: only a logit 100 above it could spoil the sums, and shows in them.
+            Eight<T> head;
+            float top = -INFINITY;
+            if (mine < bytes) {
+                head.load(here + mine, mine + 512u < bytes);
+                top = head.top();
+            }
+            st.R = __reduce_max_sync(0xFFFFFFFFu, __float2int_rn(top * c));
+            bool sound = false;
+            if (st.R > kNoRef && st.R <= kMaxRef) {
+                const typename Eight<T>::Floor floor = Eight<T>::floor_of(((float)st.R - 200.0f) * inv_c);
+                minus_ref = pair(-(float)st.R, -(float)st.R);
+#pragma unroll 1
+                for (uint32_t at = mine; at < bytes; at += kStep * (uint32_t)sizeof(T)) {
+                    Eight<T> x;
+                    x.load(here + at, at + 512u < bytes);
+                    add(x, floor);
+                }
+                st.s = total(s2);
+                st.u = total(u2);
+                sound = __all_sync(0xFFFFFFFFu, st.s < 0x1p100f);
+            }
+            if (!sound) {  // a reference of each lane's own, raised as it goes
+                st = Stats{kNoRef, 0.0f, 0.0f};
+                s2 = u2 = 0;
+                float limit = (float)(kNoRef + 64) * inv_c;
+                typename Eight<T>::Floor floor = Eight<T>::floor_of((float)(kNoRef - 200) * inv_c);
+                minus_ref = pair(-(float)kNoRef, -(float)kNoRef);
+#pragma unroll 1
+                for (uint32_t at = mine; at < bytes; at += kStep * (uint32_t)sizeof(T)) {
+                    Eight<T> x;
+                    x.load(here + at, at + 512u < bytes);
+                    top = x.top();
+                    if (top > limit) {
+                        st.s = total(s2);
+                        st.u = total(u2);
+                        raise(st, __float2int_rn(top * c));
+                        s2 = pair(st.s, 0.0f);
+                        u2 = pair(st.u, 0.0f);
+                        const float ref = (float)st.R;
+                        limit = (ref + 64.0f) * inv_c;
+                        floor = Eight<T>::floor_of((ref - 200.0f) * inv_c);
+                        minus_ref = pair(-ref, -ref);
+                    }
+                    add(x, floor);
+                }
+                st.s = total(s2);
+                st.u = total(u2);
             }
             if (hit >= r.lo && hit < r.hi)
                 l_hit = to_float(slice[hit - r.lo]);
             if (MODE == kForward || !a.dlogits)
                 refill();
-            const float2 s = halves(s2), u = halves(u2);
-            st.s = s.x + s.y;
-            st.u = u.x + u.y;
         }
         float l_token = 0.0f;
         const bool leads = ALONE || warp == 0;
@@ -616,6 +647,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) row_kernel(const RowArgs
         exchange();
         if (leads) {
             if (st.R > kNoRef && st.R <= kMaxRef) {
+                // bring a large sum to [1, 2): the gradient's factors are quotients by it
+                raise(st, st.R + max((int)(__float_as_uint(st.s) >> 23 & 0xFFu) - 127, 0));
                 finish(false, 0.0f);
             } else {
                 gr.exact = 1u;
@@ -678,28 +711,31 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) row_kernel(const RowArgs
                     if (edge_at(r, v) && v >= r.skip && v < r.end)
                         out[v] = slope(v);
                 }
+                const uint32_t start = (r.from - r.lo) * (uint32_t)sizeof(T) + (uint32_t)lane * 16u;
+                const uint32_t stop = (r.to - r.lo) * (uint32_t)sizeof(T);
+                T *to = out + r.from + lane * N;
                 if (gr.q1 != 0.0f) {
 #pragma unroll 1
-                    for (uint32_t v = r.from + lane * N; v < r.to; v += kStep) {
+                    for (uint32_t at = start; at < stop; at += kStep * (uint32_t)sizeof(T), to += kStep) {
                         Eight<T> x;
-                        x.load(here + (size_t)(v - r.lo) * sizeof(T), v + 32 * N < r.to);
+                        x.load(here + at, at + 512u < stop);
                         x.raise_to(floor);
 #pragma unroll
                         for (int j = 0; j < 4; j++) {
                             const f32x2 z = fma2(x.get(j), c2, minus_ref);
                             x.set(j, mul2(exp2_2(z), fma2(minus_q1, z, minus_q0)));
                         }
-                        x.store(out + v, v + 32 * N < r.to);
+                        x.store(to, at + 512u < stop);
                     }
                 } else {  // no entropy term
 #pragma unroll 1
-                    for (uint32_t v = r.from + lane * N; v < r.to; v += kStep) {
+                    for (uint32_t at = start; at < stop; at += kStep * (uint32_t)sizeof(T), to += kStep) {
                         Eight<T> x;
-                        x.load(here + (size_t)(v - r.lo) * sizeof(T), v + 32 * N < r.to);
+                        x.load(here + at, at + 512u < stop);
 #pragma unroll
                         for (int j = 0; j < 4; j++)
                             x.set(j, mul2(exp2_2(fma2(x.get(j), c2, minus_ref)), minus_q0));
-                        x.store(out + v, v + 32 * N < r.to);
+                        x.store(to, at + 512u < stop);
                     }
                 }
                 // the token, by the lane that has stored its vector

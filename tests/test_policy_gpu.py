@@ -10,7 +10,8 @@ at most E = 2^-22 + 0.37 x 2^-22 + 92 x 2^-24 < 6e-6: the log-probability is
 off by E + 2^-24 |lp|, the entropy by E (1 + sum p |d|) + 2^-24 H, and an
 element of the gradient, with the coefficient's own error from lp, by
 p |coefficient| (2 E + 2^-22 |d|) + 2^-23 of what is added, + half a step of its
-type.  Where log p and H cancel (a vocabulary of one: both are 0) their own
+type, and by 2^-126 |coefficient| where an exponential below the normal range is
+flushed to 0.  Where log p and H cancel (a vocabulary of one: both are 0) their own
 errors stay: p |dentropy| (E + E (1 + sum p |d|)) more.  An exponent of the policy loss magnifies lp's error by its own value."""
 import math
 
@@ -43,6 +44,7 @@ def grad64(p, logp, d, h, tokens, g, gh, t, dtype):
     spread = (p * torch.where(p == 0, 0.0, d).abs()).sum(1)
     off = size * (2 * E + 2.0 ** -22 * torch.where(p == 0, 0.0, d).abs())
     off += p * (gh.abs() * E * (2 + spread))[:, None]
+    off += 2.0 ** -126 * (g.abs()[:, None] + gh.abs()[:, None] * (logp.abs() + h.abs()[:, None]))
     hit = tokens.long()[:, None]
     ref.scatter_add_(1, hit, g[:, None])
     off.scatter_add_(1, hit, g.abs()[:, None] * 2.0 ** -23)
@@ -178,6 +180,26 @@ def test_logprobs_rows_skipped_and_bad_tokens(pkg, cuda):
     assert error.item() == 1
     assert bool((grad[1:3] == 0).all()) and bool((grad[[0, 3]] != 0).any())
     check_forward(pkg, logits[[0, 3]].contiguous(), tokens[[0, 3]].contiguous(), 1.0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("R,V", [(700, 900), (6, 9000)])
+@pytest.mark.parametrize("step", [30.0, 60.0, 68.0, 72.0, 200.0])
+def test_logprobs_of_rows_in_steps(pkg, cuda, R, V, dtype, step):
+    """Rows that rise by `step` and fall again, so that what a warp sees first is far below or
+    far above the row's maximum (in base 2: up to 288 either way); with gradients of 1e-7."""
+    logits, tokens = logits_of(cuda, R, V, dtype, 41)
+    at = torch.arange(V, device=cuda)
+    logits += (step * ((at // 97) % 2)).to(dtype)
+    logits[1::2] -= (step * (at < V // 3)).to(dtype)
+    tokens[::3] = torch.where(at % 194 > 97, logits[::3], -1e30).argmax(1).to(torch.int32)
+    check_forward(pkg, logits, tokens, 1.0)
+    check_backward(pkg, logits, tokens, 1.0)
+    p, logp, d, _, h, _ = rows64(logits, tokens, 1.0)
+    g = torch.full((R,), 1e-7, device=cuda)
+    ref, off = grad64(p, logp, d, h, tokens, g.double(), g.double(), 1.0, dtype)
+    got = pkg.token_logprobs_backward(logits, tokens, g, g)
+    assert bool(((got.double() - ref).abs() <= off).all())
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
