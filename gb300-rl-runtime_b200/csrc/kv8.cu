@@ -947,13 +947,14 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) kv8_decode_kernel(con
         const uint32_t s = i % kStages;
         const uint32_t both = i < n_pairs ? have >> (2u * i) & 3u : 4u;
         if (both) {
-            // After an expired wait nothing is issued any more; what is in flight is
-            // waited for, each entry again with a limit.
-            if (!__all_sync(0xFFFFFFFFu, rt::mbar_wait_bounded(rt::smem_u32(&bars[warp][s]),
-                                                               (phases >> s) & 1u, kWaitLimitNs))) {
+            // After an expired wait nothing is issued any more; what is in flight, this
+            // entry included, is waited for, again with a limit.
+            const uint32_t bar = rt::smem_u32(&bars[warp][s]), phase = (phases >> s) & 1u;
+            if (!__all_sync(0xFFFFFFFFu, rt::mbar_wait_bounded(bar, phase, kWaitLimitNs))) {
                 if (lane == 0)
                     flag_error(a.error, kErrTimeout);
                 limit = 0;
+                rt::mbar_wait_bounded(bar, phase, kWaitLimitNs);
             }
             phases ^= 1u << s;
             const uint8_t *base = slots + s * kEntryBytes;
@@ -1058,6 +1059,9 @@ __global__ void __launch_bounds__(WARPS == 1 ? 256 : WARPS * 32) kv8_merge_kerne
     __shared__ float4 warp_o[WARPS][32];
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, G = a.G;
     const uint64_t item = WARPS == 1 ? blockIdx.x * 8ull + warp : blockIdx.x;
+    // every CTA waits, also those without a part in it: this kernel's end stands for
+    // both kernels' to what follows
+    rt::grid_dep_wait();
     if (item >= (uint64_t)a.num_seqs * a.num_kv_heads * G)
         return;
     const uint64_t row = item / G;
@@ -1069,7 +1073,6 @@ __global__ void __launch_bounds__(WARPS == 1 ? 256 : WARPS * 32) kv8_merge_kerne
     if (n < 2)
         return;
     const uint64_t first = row * a.max_chunks * G + item % G;
-    rt::grid_dep_wait();
     // all maxima -infinity: no page was read, or all scores were NaN
     auto weight = [](float x, float top) { return top == -INFINITY ? 1.0f : rt::fast_exp2(x - top); };
     float m = -INFINITY, l = 0.0f;
@@ -1174,7 +1177,7 @@ int check_attn(const rt_kv8_attn_params_t *p)
     }
     if (!p->num_kv_heads || !p->num_q_heads || p->num_q_heads % p->num_kv_heads ||
         p->num_q_heads / p->num_kv_heads > 8u || !format_ok(p->format) ||
-        p->chunk_pages > kMaxChunkPages || !(fabsf(p->scale) <= 3.4e38f) ||
+        p->chunk_pages > kMaxChunkPages || !(fabsf(p->scale) <= 2e38f) ||
         p->q_stride < (uint64_t)p->num_q_heads * 128u || p->q_stride % 8u ||
         p->max_seq_len > 0x7FFFFFFFu || (p->max_seq_len >> 4) > p->max_pages_per_seq) {
         rt::set_error("kv8_decode_attention: 1..8 query heads to a KV head (%u / %u), format e4m3 "
@@ -1212,7 +1215,9 @@ extern "C" int rt_kv8_append(const rt_kv8_append_params_t *p, const void *k, con
                       ">= num_kv_heads * 128 and multiples of 8");
         return RT_EINVAL;
     }
-    if (!k || !v || !cu_tokens || !seq_lens || !page_table || !pages || !scales || !tail) {
+    // no page table or no arena: none of it is read
+    if (!k || !v || !cu_tokens || !seq_lens || (!page_table && p->max_pages_per_seq) ||
+        ((!pages || !scales) && p->arena_pages) || !tail) {
         rt::set_error("kv8_append: null argument");
         return RT_EINVAL;
     }
@@ -1285,7 +1290,8 @@ extern "C" int rt_kv8_decode_attention(const rt_kv8_attn_params_t *p, const void
         return rc;
     if (p->num_seqs == 0)
         return RT_OK;
-    if (!q || !pages || !scales || !tail || !page_table || !seq_lens || !out) {
+    if (!q || ((!pages || !scales) && p->arena_pages) || !tail ||
+        (!page_table && p->max_pages_per_seq) || !seq_lens || !out) {
         rt::set_error("kv8_decode_attention: null argument");
         return RT_EINVAL;
     }

@@ -485,3 +485,65 @@ def test_two_streams_at_once(pkg, cuda):
             for _ in range(20)]
     torch.cuda.synchronize()
     assert all(torch.equal(o, want) for pair in outs for o in pair)
+
+
+@pytest.mark.parametrize("heads,G", [(1, 1), (8, 4)])
+def test_what_follows_waits_for_the_whole_call(pkg, cuda, heads, G):
+    """A bound that provides for splits where no sequence has any: the merge has nothing to
+    do, and what the stream does next must still find the outputs done."""
+    lens = [1500, 1530, 3, 1536]
+    case = make(pkg, cuda, lens, heads, G, "s8", seed=21)
+    table = np.full((4, 4096), -7, np.int32)
+    table[:, :case[4].shape[1]] = case[4]
+    case = (*case[:4], table)
+    want = attend(pkg, cuda, *case, lens)
+    td, ld = torch.from_numpy(table).to(cuda), torch.tensor(lens, dtype=torch.int32, device=cuda)
+    out, seen = torch.zeros_like(want), []
+    for _ in range(50):
+        out.fill_(-1.0)
+        pkg.kv8_decode_attention(*case[:4], td, ld, 65535, out=out, chunk_pages=96)
+        seen.append(out.clone())
+    torch.cuda.synchronize()
+    check(want, *case, lens)
+    for s in seen:
+        check(s, *case, lens)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "s8"])
+def test_sequences_without_a_page(pkg, cuda, fmt):
+    """An arena of no pages and a page table of no columns: tails alone."""
+    g = torch.Generator(device=cuda).manual_seed(22)
+    lens = [15, 0, 1, 9]
+    k, v = torch.randn(2, sum(lens), 2, 128, generator=g, device=cuda).bfloat16()
+    bufs = pkg.kv8_cache(0, 4, 2, fmt, cuda)
+    table = np.zeros((4, 0), np.int32)
+    do_append(pkg, cuda, bufs, k, v, [0] * 4, lens, table)
+    q = torch.randn(4, 8, 128, generator=g, device=cuda).bfloat16()
+    got = attend(pkg, cuda, q, *bufs, table, lens)
+    check(got, q, *bufs, table, lens)
+    # a token more would need a page
+    error = torch.zeros(1, dtype=torch.int32, device=cuda)
+    pkg.kv8_append(k[:1], v[:1], torch.tensor([0, 1, 1, 1, 1], dtype=torch.int32, device=cuda),
+                   torch.tensor(lens, dtype=torch.int32, device=cuda),
+                   torch.from_numpy(table).to(cuda), *bufs, error=error)
+    assert error.item() == 1
+
+
+def test_padded_tokens_and_shared_pages(pkg, cuda):
+    """Rows behind the last sequence's (NaN here) are not read; two sequences read the same
+    pages of a common prefix, one of them twice."""
+    g = torch.Generator(device=cuda).manual_seed(23)
+    k, v = torch.full((2, 64, 2, 128), float("nan"), device=cuda).bfloat16()
+    k[:40], v[:40] = torch.randn(2, 40, 2, 128, generator=g, device=cuda).bfloat16()
+    bufs = cache(pkg, cuda, "s8", 4, 2, 2, 6)
+    model = Model(*bufs, "s8")
+    table = tables([32, 8], 4, 7)
+    do_append(pkg, cuda, bufs, k, v, [0, 0], [32, 8], table)
+    rows = np.stack([bf16(k), bf16(v)], 2)
+    model.append(0, 0, rows[:32], table[0])
+    model.append(1, 0, rows[32:40], table[1])
+    model.check(*bufs)
+    table[1, :3] = table[0, [0, 1, 0]]
+    lens = [32, 56]
+    q = torch.randn(2, 8, 128, generator=g, device=cuda).bfloat16()
+    check(attend(pkg, cuda, q, *bufs, table, lens), q, *bufs, table, lens)
