@@ -334,10 +334,15 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) row_kernel(const RowArgs
         }
     };
     uint32_t phase = 0;
+    // After an expired wait the copy is waited for once more, again with a limit.
     auto arrived = [&](const Span &r) {
         if (r.from < r.to) {
-            if (!rt::mbar_wait_bounded(rt::smem_u32(&bars[warp]), phase, kWaitLimitNs) && a.error)
-                atomicCAS(a.error, 0, kErrTimeout);
+            const uint32_t bar = rt::smem_u32(&bars[warp]);
+            if (!rt::mbar_wait_bounded(bar, phase, kWaitLimitNs)) {
+                if (a.error)
+                    atomicCAS(a.error, 0, kErrTimeout);
+                rt::mbar_wait_bounded(bar, phase, kWaitLimitNs);
+            }
             phase ^= 1u;
         }
     };
@@ -427,6 +432,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) row_kernel(const RowArgs
         }
     }
     uint32_t exchanges = 0;
+    bool late = false;  // a statistics wait has expired (warp 0)
     if (early && !(todo & 1u))
         arrived(r);
     if (!ALONE)
@@ -468,7 +474,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) row_kernel(const RowArgs
         {
             arrived(r);
             const uint32_t bytes = (r.hi - r.lo) * (uint32_t)sizeof(T), mine = (uint32_t)lane * 16u;
-            f32x2 s2 = 0, u2 = 0, minus_ref;
+            f32x2 s2, u2, minus_ref;
             auto add = [&](Eight<T> &x, typename Eight<T>::Floor floor) {
                 x.raise_to(floor);
 #pragma unroll
@@ -479,58 +485,46 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) row_kernel(const RowArgs
                 }
             };
             auto total = [&](f32x2 v) { return halves(v).x + halves(v).y; };
-            // The warp's first vectors give its reference.  It does not have to be the
-            // maximum: only a logit 100 above it could spoil the sums, and shows in them.
+            // The warp's first vectors, and the token, which is often the row's peak, give its
+            // reference.  It does not have to be the maximum: a logit so far above it that z and u lose digits (by more than 12 in
+            // base 2) shows in the sums, and then the region's maximum is taken.
             Eight<T> head;
             float top = -INFINITY;
             if (mine < bytes) {
                 head.load(here + mine, mine + 512u < bytes);
                 top = head.top();
             }
-            st.R = __reduce_max_sync(0xFFFFFFFFu, __float2int_rn(top * c));
-            bool sound = false;
-            if (st.R > kNoRef && st.R <= kMaxRef) {
+            if (hit >= r.lo && hit < r.hi) {
+                l_hit = to_float(slice[hit - r.lo]);
+                top = fmaxf(top, l_hit);
+            }
+            // Statistics of the region for the lanes' largest `top`.
+            auto sums = [&]() {
+                st = Stats{max(__reduce_max_sync(0xFFFFFFFFu, __float2int_rn(top * c)), kNoRef), 0.0f, 0.0f};
+                if (st.R > kMaxRef)
+                    return;
                 const typename Eight<T>::Floor floor = Eight<T>::floor_of(((float)st.R - 200.0f) * inv_c);
                 minus_ref = pair(-(float)st.R, -(float)st.R);
-#pragma unroll 1
-                for (uint32_t at = mine; at < bytes; at += kStep * (uint32_t)sizeof(T)) {
-                    Eight<T> x;
-                    x.load(here + at, at + 512u < bytes);
-                    add(x, floor);
-                }
-                st.s = total(s2);
-                st.u = total(u2);
-                sound = __all_sync(0xFFFFFFFFu, st.s < 0x1p100f);
-            }
-            if (!sound) {  // a reference of each lane's own, raised as it goes
-                st = Stats{kNoRef, 0.0f, 0.0f};
                 s2 = u2 = 0;
-                float limit = (float)(kNoRef + 64) * inv_c;
-                typename Eight<T>::Floor floor = Eight<T>::floor_of((float)(kNoRef - 200) * inv_c);
-                minus_ref = pair(-(float)kNoRef, -(float)kNoRef);
 #pragma unroll 1
                 for (uint32_t at = mine; at < bytes; at += kStep * (uint32_t)sizeof(T)) {
                     Eight<T> x;
                     x.load(here + at, at + 512u < bytes);
-                    top = x.top();
-                    if (top > limit) {
-                        st.s = total(s2);
-                        st.u = total(u2);
-                        raise(st, __float2int_rn(top * c));
-                        s2 = pair(st.s, 0.0f);
-                        u2 = pair(st.u, 0.0f);
-                        const float ref = (float)st.R;
-                        limit = (ref + 64.0f) * inv_c;
-                        floor = Eight<T>::floor_of((ref - 200.0f) * inv_c);
-                        minus_ref = pair(-ref, -ref);
-                    }
                     add(x, floor);
                 }
                 st.s = total(s2);
                 st.u = total(u2);
+            };
+            sums();
+            if (__builtin_expect(!__all_sync(0xFFFFFFFFu, st.s < 4096.0f), 0)) {
+#pragma unroll 1
+                for (uint32_t at = mine; at < bytes; at += kStep * (uint32_t)sizeof(T)) {
+                    Eight<T> x;
+                    x.load(here + at, at + 512u < bytes);
+                    top = fmaxf(top, x.top());
+                }
+                sums();
             }
-            if (hit >= r.lo && hit < r.hi)
-                l_hit = to_float(slice[hit - r.lo]);
             if (MODE == kForward || !a.dlogits)
                 refill();
         }
@@ -553,8 +547,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) row_kernel(const RowArgs
                            make_uint4((uint32_t)st.R, __float_as_uint(st.s), __float_as_uint(st.u),
                                       __float_as_uint(l_hit)));
             if (warp == 0) {
-                if (!rt::mbar_wait_bounded(bar, exchanges >> 1 & 1u, kWaitLimitNs) && a.error)
-                    atomicCAS(a.error, 0, kErrTimeout);
+                if (!rt::mbar_wait_bounded(bar, exchanges >> 1 & 1u, kWaitLimitNs)) {
+                    late = true;
+                    if (a.error)
+                        atomicCAS(a.error, 0, kErrTimeout);
+                }
                 st = Stats{INT32_MIN, 0.0f, 0.0f};
                 l_token = 0.0f;
                 for (uint32_t e = lane; e < n_entries; e += 32) {
@@ -751,6 +748,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) row_kernel(const RowArgs
         r = next;
         edge = next_edge;
     }
+    // Statistics that have not come are still under way to this CTA's memory: it stays
+    // until the cluster's other CTAs are through.
+    if (!ALONE && __any_sync(0xFFFFFFFFu, late)) {
+        cluster_arrive();
+        cluster_wait();
+    }
 }
 
 // Weighted sums over the rows' records, in fp64 and a fixed order: one cluster of
@@ -765,7 +768,7 @@ __global__ void __launch_bounds__(512) policy_stats_kernel(const rt_policy_row_t
     cluster_arrive();
     rt::grid_dep_wait();  // the rows' records are there
     double sum[5] = {0, 0, 0, 0, 0};
-    for (uint32_t r = rank * 512u + threadIdx.x; r < n; r += kStatsCtas * 512u) {
+    for (uint64_t r = rank * 512u + threadIdx.x; r < n; r += kStatsCtas * 512u) {
         const float4 x = reinterpret_cast<const float4 *>(rows + r)[0];
         const float4 y = reinterpret_cast<const float4 *>(rows + r)[1];
         const double w = y.w;

@@ -203,6 +203,28 @@ def test_logprobs_of_rows_in_steps(pkg, cuda, R, V, dtype, step):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("R,V", [(700, 2000), (40, 32000)])
+@pytest.mark.parametrize("gap", [3.0, 6.0, 11.0, 16.0, 30.0, 60.0])
+def test_logprobs_of_peaked_rows(pkg, cuda, R, V, dtype, gap):
+    """One element far above the others, wherever it lies, which is the row's token or not.
+    With gaps above 16 the others are less than 2^-7 of the sum (32000 e^(1/2) e^-16), and what
+    the log-probability is off by is the one large summand's: 2^-22 of its exp2, 2^-22 of its
+    exponent's rounding (below 12 in base 2), and at most 92 additions of 2^-24."""
+    logits, tokens = logits_of(cuda, R, V, dtype, 47, std=1.0)
+    logits.clamp_(-5, 5)
+    tokens[:] = torch.linspace(0, V - 1, R, device=cuda).to(torch.int32)
+    logits[torch.arange(R, device=cuda), tokens.long()] = 5.0 + gap
+    tokens[::2] = (tokens[::2] * 7 + 1) % V
+    check_forward(pkg, logits, tokens, 1.0)
+    check_backward(pkg, logits, tokens, 1.0)
+    if gap > 16:
+        lp, _ = pkg.token_logprobs(logits, tokens)
+        want = rows64(logits, tokens, 1.0)[3]
+        bound = 2.0 ** -21 + 92 * 2.0 ** -24 + 2.0 ** -24 * want.abs()
+        assert bool(((lp.double() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("R,V", [(900, 555), (60, 20011)])
 def test_logprobs_awkward_rows_among_others(pkg, cuda, R, V, dtype):
     """Rows without a number, masked rows, rows of logits in the millions (of which one at the
