@@ -33,6 +33,7 @@ constexpr uint32_t kMaxCluster = 8;
 constexpr uint32_t kMaxRows = 32;  // of a group, one to a lane
 constexpr uint32_t kMaxVocab = 262144;
 constexpr uint64_t kWaitLimitNs = 2000000000ull;
+constexpr uint32_t kMaxSmem = 224 * 1024;    // of a CTA, at most
 constexpr uint32_t kSmemTarget = 72 * 1024;  // of a CTA: three to an SM
 
 struct RowArgs {
@@ -828,8 +829,9 @@ int launch_rows(RowArgs &a, uint32_t k, cudaStream_t stream, const char *what)
     a.region = ((a.vocab + N - 1 + N - 1) / N + warps - 1) / warps * N;
     const uint32_t one = a.region * kRowWarps * esz;
     const size_t bytes = (size_t)one;
+    // the same value in every call: host threads may set it at once
     cudaError_t e = cudaFuncSetAttribute(row_kernel<T, MODE, ALONE>,
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMaxSmem);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(k);
     cfg.blockDim = dim3(kThreads);

@@ -484,3 +484,29 @@ def test_rows_beyond_32_bits(pkg, cuda):
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
     want = pkg.token_logprobs_backward(small, tokens, g, g)
     assert torch.equal(pkg.token_logprobs_backward(logits, tokens, g, g, dlogits=logits), want)
+
+
+def test_calls_of_two_threads(pkg, cuda):
+    """Two host threads with rows of different lengths, each on its own stream."""
+    import threading
+    shapes = [(64, 32000), (64, 131077)]
+    cases = [logits_of(cuda, R, V, torch.float32, V) for R, V in shapes]
+    want = [pkg.token_logprobs(*c) for c in cases]
+    torch.cuda.synchronize()
+    wrong, streams = [], [torch.cuda.Stream() for _ in shapes]
+
+    def work(i):
+        try:
+            got = [pkg.token_logprobs(*cases[i], stream=streams[i]) for _ in range(200)]
+            streams[i].synchronize()
+            wrong.extend(1 for a, b in got
+                         if not (torch.equal(a, want[i][0]) and torch.equal(b, want[i][1])))
+        except Exception as e:
+            wrong.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
