@@ -470,43 +470,44 @@ def _need(ok, what):
 
 
 def _same_device(first, *others):
-    """Every tensor given lies on the first one's CUDA device."""
-    dev = first.device
-    if dev.type != "cuda":
+    """The index of the CUDA device that every tensor given lies on."""
+    index = first.get_device()
+    if index < 0:
         raise ValueError("tensors must be on a CUDA device")
     for t in others:
-        if t is not None and t.device != dev:
+        if t is not None and t.get_device() != index:
             raise ValueError("tensors must be on one device")
-    return dev
+    return index
 
 
 _HERE = contextlib.nullcontext()
-_torch = None
+_torch = _F32 = _BF16 = _I32 = _U32 = None
 _DTYPES = {}
 _KV8_FORMATS = {}
 
 
 def _tm():
     """torch, imported at the first call that needs it."""
-    global _torch
+    global _torch, _F32, _BF16, _I32, _U32
     if _torch is None:
         import torch
+        _F32, _BF16, _I32, _U32 = torch.float32, torch.bfloat16, torch.int32, torch.uint32
         _DTYPES.update({torch.float32: RT_DTYPE_F32, torch.bfloat16: RT_DTYPE_BF16})
         _KV8_FORMATS.update({torch.float8_e4m3fn: RT_KV8_E4M3, torch.int8: RT_KV8_S8})
         _torch = torch
     return _torch
 
 
-def _on(dev, stream):
+def _on(index, stream):
     """A context in which the tensors' device is current, and `stream` where one is given (so
     that what is allocated inside belongs to the stream that uses it), and the stream's handle."""
-    torch = _torch
+    cuda = _torch.cuda
     if stream is not None:
-        _need(stream.device == dev, "the stream is another device's")
-        return torch.cuda.stream(stream), stream.cuda_stream
-    if torch.cuda.current_device() == dev.index:
-        return _HERE, torch._C._cuda_getCurrentRawStream(dev.index)
-    return torch.cuda.device(dev), torch.cuda.current_stream(dev).cuda_stream
+        _need(stream.device.index == index, "the stream is another device's")
+        return cuda.stream(stream), stream.cuda_stream
+    if _torch._C._cuda_getDevice() == index:
+        return _HERE, _torch._C._cuda_getCurrentRawStream(index)
+    return cuda.device(index), cuda.current_stream(index).cuda_stream
 
 
 def _error_word(error):
@@ -517,24 +518,25 @@ def _error_word(error):
 
 
 def _int_array(t, shape, what):
-    if t.dtype != _torch.int32 or t.shape != shape or not t.is_contiguous():
-        raise ValueError(f"{what}: contiguous int32 {tuple(shape)}, got {t.dtype} "
-                         f"{tuple(t.shape)}")
-    return t.data_ptr()
+    if t.dtype is _I32 and t.shape == shape and t.is_contiguous():
+        return t.data_ptr()
+    raise ValueError(f"{what}: contiguous int32 {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
 
 
 def _kv8_cache(pages, scales, tail, num_seqs):
     """(format, pages, KV heads) of a cache's buffers, checked."""
-    torch = _torch
     fmt = _KV8_FORMATS.get(pages.dtype)
-    _need(fmt is not None, "pages: float8_e4m3fn or int8")
-    _need(pages.dim() == 4 and pages.is_contiguous(), "pages: contiguous [n, kv heads, 2, 2048]")
-    n, h, planes, size = pages.shape
-    _need(planes == 2 and size == KV8_PLANE_BYTES, "pages: contiguous [n, kv heads, 2, 2048]")
-    _need(scales.dtype == torch.float32 and scales.shape == (n, h, 2) and scales.is_contiguous(),
-          "scales: contiguous float32 [n, kv heads, 2]")
-    _need(tail.dtype == torch.bfloat16 and tail.shape == (num_seqs, h, 2, 16, 128)
-          and tail.is_contiguous(), "tail: contiguous bfloat16 [sequences, kv heads, 2, 16, 128]")
+    if fmt is None:
+        raise ValueError("pages: float8_e4m3fn or int8")
+    shape = pages.shape
+    if len(shape) != 4 or shape[2] != 2 or shape[3] != KV8_PLANE_BYTES or not pages.is_contiguous():
+        raise ValueError("pages: contiguous [n, kv heads, 2, 2048]")
+    n, h = shape[0], shape[1]
+    if scales.dtype is not _F32 or scales.shape != (n, h, 2) or not scales.is_contiguous():
+        raise ValueError("scales: contiguous float32 [n, kv heads, 2]")
+    if (tail.dtype is not _BF16 or tail.shape != (num_seqs, h, 2, 16, 128)
+            or not tail.is_contiguous()):
+        raise ValueError("tail: contiguous bfloat16 [sequences, kv heads, 2, 16, 128]")
     return fmt, n, h
 
 
@@ -549,26 +551,33 @@ def kv8_cache(n_pages, num_seqs, num_kv_heads, format="e4m3", device="cuda"):
             torch.zeros(num_seqs, num_kv_heads, 2, 16, 128, dtype=torch.bfloat16, device=device))
 
 
+def _width(page_table):
+    if page_table.dim() != 2:
+        raise ValueError("page_table: int32 [sequences, P]")
+    return page_table.shape[1]
+
+
 def kv8_append(k, v, cu_tokens, seq_lens, page_table, pages, scales, tail, error=None,
                stream=None):
     """rt_kv8_append: tokens cu_tokens[b] .. cu_tokens[b + 1] of k and v (bf16 or fp32
     [T, kv heads, 128], any token stride that is a multiple of 8) behind the seq_lens[b]
     tokens that sequence b has.  cu_tokens int32 [B + 1], seq_lens int32 [B], page_table
     int32 [B, P]; pages, scales and tail as kv8_cache makes them.  seq_lens is not advanced."""
-    _tm()
+    if _torch is None:
+        _tm()
     B = seq_lens.shape[0]
     dev = _same_device(pages, k, v, cu_tokens, seq_lens, page_table, scales, tail, error)
     fmt, n_pages, h = _kv8_cache(pages, scales, tail, B)
     dtype = _DTYPES.get(k.dtype)
-    _need(dtype is not None and v.dtype == k.dtype, "k, v: both bfloat16 or both float32")
+    if dtype is None or v.dtype is not k.dtype:
+        raise ValueError("k, v: both bfloat16 or both float32")
     T = k.shape[0]
     shape, row = (T, h, 128), h * 128
     k_stride, k_head, k_dim = k.stride() if k.shape == shape else (0, 0, 0)
     v_stride, v_head, v_dim = v.stride() if v.shape == shape else (0, 0, 0)
-    _need(k_dim == 1 and v_dim == 1 and (h == 1 or (k_head == 128 and v_head == 128)),
-          "k, v: [tokens, kv heads, 128] with contiguous heads")
-    _need(page_table.dim() == 2 and page_table.shape[0] == B, "page_table: int32 [sequences, P]")
-    P = page_table.shape[1]
+    if k_dim != 1 or v_dim != 1 or (h != 1 and (k_head != 128 or v_head != 128)):
+        raise ValueError("k, v: [tokens, kv heads, 128] with contiguous heads")
+    P = _width(page_table)
     p = rt_kv8_append_params_t(B, h, T, P, n_pages, k_stride if T > 1 else row,
                                v_stride if T > 1 else row, fmt, dtype)
     cu, lens = _int_array(cu_tokens, (B + 1,), "cu_tokens"), _int_array(seq_lens, (B,), "seq_lens")
@@ -585,22 +594,23 @@ def kv8_decode_attention(q, pages, scales, tail, page_table, seq_lens, max_seq_l
     """rt_kv8_decode_attention: q bf16 [B, Hq, 128] over the cache of kv8_append; returns
     fp32 [B, Hq, 128].  max_seq_len bounds every seq_lens[b].  workspace: uint8, by default
     a new one (from torch's allocator, on the current stream)."""
-    torch = _tm()
+    if _torch is None:
+        _tm()
     B = seq_lens.shape[0]
     dev = _same_device(q, pages, scales, tail, page_table, seq_lens, out, workspace, error)
     fmt, n_pages, h = _kv8_cache(pages, scales, tail, B)
-    _need(q.dtype == torch.bfloat16 and q.dim() == 3, "q: bfloat16 [sequences, heads, 128]")
+    if q.dtype is not _BF16 or q.dim() != 3:
+        raise ValueError("q: bfloat16 [sequences, heads, 128]")
     n, Hq, dim = q.shape
     q_stride, q_head, q_dim = q.stride()
-    _need(n == B and dim == 128 and q_dim == 1 and (Hq == 1 or q_head == 128),
-          "q: bfloat16 [sequences, heads, 128] with contiguous heads")
-    _need(out is None or (out.dtype == torch.float32 and out.shape == (B, Hq, 128)
-                          and out.is_contiguous()),
-          "out: contiguous float32 [sequences, heads, 128]")
-    _need(page_table.dim() == 2 and page_table.shape[0] == B, "page_table: int32 [sequences, P]")
-    P = page_table.shape[1]
-    _need(0 <= max_seq_len <= 0x7FFFFFFF and 0 <= chunk_pages <= 128,
-          "max_seq_len 0 .. 2^31 - 1, chunk_pages 0 .. 128")
+    if n != B or dim != 128 or q_dim != 1 or (Hq != 1 and q_head != 128):
+        raise ValueError("q: bfloat16 [sequences, heads, 128] with contiguous heads")
+    if out is not None and (out.dtype is not _F32 or out.shape != (B, Hq, 128)
+                            or not out.is_contiguous()):
+        raise ValueError("out: contiguous float32 [sequences, heads, 128]")
+    P = _width(page_table)
+    if not (0 <= max_seq_len <= 0x7FFFFFFF and 0 <= chunk_pages <= 128):
+        raise ValueError("max_seq_len 0 .. 2^31 - 1, chunk_pages 0 .. 128")
     p = rt_kv8_attn_params_t(B, Hq, h, P, max_seq_len, fmt, n_pages,
                              q_stride if B > 1 else Hq * 128,
                              128 ** -0.5 if scale is None else scale, chunk_pages)
@@ -609,13 +619,15 @@ def kv8_decode_attention(q, pages, scales, tail, page_table, seq_lens, max_seq_l
     ctx, s = _on(dev, stream)
     with ctx:
         if out is None:
-            out = torch.empty((B, Hq, 128), dtype=torch.float32, device=dev)
-        size = lib().rt_kv8_attn_workspace_bytes(ref)
-        if size and workspace is None:
-            workspace = torch.empty(size, dtype=torch.uint8, device=dev)
-        elif workspace is not None:
+            out = q.new_empty((B, Hq, 128), dtype=_F32)
+        native = lib()
+        if workspace is not None:
             size = workspace.numel() * workspace.element_size()
-        check(lib().rt_kv8_decode_attention(
+        else:
+            size = native.rt_kv8_attn_workspace_bytes(ref)
+            if size:
+                workspace = q.new_empty(size, dtype=_torch.uint8)
+        check(native.rt_kv8_decode_attention(
             ref, q.data_ptr(), pages.data_ptr(), scales.data_ptr(), tail.data_ptr(), table, lens,
             out.data_ptr(), None if workspace is None else workspace.data_ptr(), size,
             _error_word(error), s), "rt_kv8_decode_attention")
@@ -1098,37 +1110,40 @@ def grpo_advantages(rewards, group, eps=1e-6, out=None, stream=None):
 
 
 def _rows_of(logits, tokens):
-    """(rows, vocab, row stride, dtype) of a matrix of logits and its tokens, checked."""
+    """(rows, vocab, row stride, dtype, tokens) of a matrix of logits and its tokens, checked."""
     dtype = _DTYPES.get(logits.dtype)
-    _need(dtype is not None and logits.dim() == 2, "logits: bfloat16 or float32 [rows, vocab]")
+    if dtype is None or logits.dim() != 2:
+        raise ValueError("logits: bfloat16 or float32 [rows, vocab]")
     R, V = logits.shape
     stride, step = logits.stride()
-    _need(V == 1 or step == 1, "logits: contiguous rows")
+    if step != 1 and V != 1:
+        raise ValueError("logits: contiguous rows")
     return R, V, (stride if R > 1 else V), dtype, _index_array(tokens, R, "tokens")
 
 
 def _float_array(t, n, what):
     if t is None:
         return None
-    if t.dtype != _torch.float32 or t.shape != (n,) or not t.is_contiguous():
-        raise ValueError(f"{what}: contiguous float32 [{n}], got {t.dtype} {tuple(t.shape)}")
-    return t.data_ptr()
+    if t.dtype is _F32 and t.shape == (n,) and t.is_contiguous():
+        return t.data_ptr()
+    raise ValueError(f"{what}: contiguous float32 [{n}], got {t.dtype} {tuple(t.shape)}")
 
 
 def _index_array(t, n, what):
     if t is None:
         return None
-    if t.dtype not in (_torch.int32, _torch.uint32) or t.shape != (n,) or not t.is_contiguous():
-        raise ValueError(f"{what}: contiguous int32 [{n}], got {t.dtype} {tuple(t.shape)}")
-    return t.data_ptr()
+    if (t.dtype is _I32 or t.dtype is _U32) and t.shape == (n,) and t.is_contiguous():
+        return t.data_ptr()
+    raise ValueError(f"{what}: contiguous int32 [{n}], got {t.dtype} {tuple(t.shape)}")
 
 
 def _gradient_of(logits, dlogits, R, V):
     """The gradient's buffer (a new one for None) and its row stride."""
     if dlogits is None:
-        return _torch.empty((R, V), dtype=logits.dtype, device=logits.device), V
-    _need(dlogits.dtype == logits.dtype and dlogits.shape == (R, V)
-          and (V == 1 or dlogits.stride(1) == 1), "dlogits: the logits' type and shape")
+        return logits.new_empty((R, V)), V
+    if (dlogits.dtype is not logits.dtype or dlogits.shape != (R, V)
+            or (V != 1 and dlogits.stride(1) != 1)):
+        raise ValueError("dlogits: the logits' type and shape")
     return dlogits, (dlogits.stride(0) if R > 1 else V)
 
 
@@ -1137,7 +1152,8 @@ def token_logprobs(logits, tokens, temperature=1.0, row_enable=None, logprobs=No
     """rt_token_logprobs: (log-probability of each row's token, entropy of each row), fp32 [R],
     of logits fp32 or bf16 [R, V] (any row stride) and tokens int32 [R].  Rows whose row_enable
     (int32 [R]) is 0 are skipped: give logprobs and entropy to know what they hold."""
-    torch = _tm()
+    if _torch is None:
+        _tm()
     R, V, stride, dtype, tok = _rows_of(logits, tokens)
     dev = _same_device(logits, tokens, row_enable, logprobs, entropy, error)
     p = rt_logprob_params_t(R, V, stride, 0, dtype, temperature,
@@ -1145,11 +1161,11 @@ def token_logprobs(logits, tokens, temperature=1.0, row_enable=None, logprobs=No
     ctx, s = _on(dev, stream)
     with ctx:
         if logprobs is None:
-            logprobs = torch.empty(R, dtype=torch.float32, device=dev)
+            logprobs = logits.new_empty(R, dtype=_F32)
         else:
             _float_array(logprobs, R, "logprobs")
         if entropy is None:
-            entropy = torch.empty(R, dtype=torch.float32, device=dev)
+            entropy = logits.new_empty(R, dtype=_F32)
         else:
             _float_array(entropy, R, "entropy")
         check(lib().rt_token_logprobs(ctypes.byref(p), logits.data_ptr(), tok, logprobs.data_ptr(),
@@ -1162,7 +1178,8 @@ def token_logprobs_backward(logits, tokens, dlogprobs, dentropy=None, temperatur
                             row_enable=None, dlogits=None, error=None, stream=None):
     """rt_token_logprobs_backward: the gradient with respect to the logits, in their type;
     dlogits may be the logits themselves."""
-    _tm()
+    if _torch is None:
+        _tm()
     R, V, stride, dtype, tok = _rows_of(logits, tokens)
     dev = _same_device(logits, tokens, dlogprobs, dentropy, row_enable, dlogits, error)
     ctx, s = _on(dev, stream)
@@ -1203,21 +1220,23 @@ def policy_loss(logits, tokens, weights, advantages, old_logprobs=None, ref_logp
     gradient.  weights fp32 [R]; advantages fp32 [S], one per rollout, with row_seq int32 [R]
     naming each row's (None: one per row); old_logprobs None: on-policy.  dlogits may be the
     logits themselves; backward=False computes the values alone.  Returns a PolicyLoss."""
-    torch = _tm()
+    if _torch is None:
+        _tm()
     R, V, stride, dtype, tok = _rows_of(logits, tokens)
     dev = _same_device(logits, tokens, weights, advantages, old_logprobs, ref_logprobs, row_seq,
                        dlogits, error)
-    _need(backward or dlogits is None, "dlogits without backward")
-    _need(advantages.dim() == 1 and (row_seq is not None or advantages.shape[0] == R),
-          "advantages: one per row without row_seq")
+    if dlogits is not None and not backward:
+        raise ValueError("dlogits without backward")
     S = advantages.shape[0]
+    if row_seq is None and S != R:
+        raise ValueError("advantages: one per row without row_seq")
     ctx, s = _on(dev, stream)
     with ctx:
         grad_stride = 0
         if backward:
             dlogits, grad_stride = _gradient_of(logits, dlogits, R, V)
-        rows = torch.empty((R, 8), dtype=torch.float32, device=dev)
-        stats = torch.empty(5, dtype=torch.float32, device=dev)
+        rows = logits.new_empty((R, 8), dtype=_F32)
+        stats = logits.new_empty(5, dtype=_F32)
         p = rt_policy_params_t(R, V, S, dtype, stride, grad_stride, temperature, clip_low,
                                clip_high, kl_coef, entropy_coef)
         check(lib().rt_policy_loss(
