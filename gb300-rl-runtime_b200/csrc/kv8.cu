@@ -8,10 +8,10 @@
 // Both move bytes: their floor is what they read and write once, at the rate of a
 // copy (6,547 GB/s measured here).  Times are of calls in a graph, inputs changing
 // from call to call, merge included.
-//   append     256 sequences x 1 token, 8 KV heads       6.8 us  (launch and the
-//                                       three dependent loads before a row's)
-//              64 prompts of 64..1,024 tokens             45 us  76% of copy
-//              4 prompts of 30,001..32,768 tokens        128 us  91%
+//   append     256 sequences x 1 token, 8 KV heads       5.3 us  (launch and the
+//                                       dependent loads before a row's)
+//              64 prompts of 64..1,024 tokens             46 us  75% of copy
+//              4 prompts of 30,001..32,768 tokens        127 us  92%
 //   attention  1 sequence of 17 tokens                   4.2 us  (latency)
 //              64 of 128..4,096, 32 heads on 8            58 us  82%
 //              256 of 512..768, 32 heads on 8             63 us  83%
@@ -194,10 +194,10 @@ __device__ __forceinline__ void store_tile(const uint2 (&x)[16], uint32_t plane,
 }
 
 // One warp per (unit, KV head), K and V; a unit is one page of one sequence that
-// the call touches.  Sequence b owns the units from cu[b] / 16 + 2 b on: n new
-// tokens behind any remainder touch at most n / 16 + 2 pages, so the ranges are
-// disjoint and a unit finds its sequence by a search of cu, 32 ways at a time,
-// without a scan over the batch.  Lane i holds dimensions 4 i .. 4 i + 3 of all 16
+// the call completes, and the first of a sequence its tail.  Sequence b owns the
+// units from cu[b] / 16 + b on: n new tokens behind a remainder of up to 15 complete
+// at most n / 16 + 1 pages, so the ranges are disjoint and a unit finds its sequence
+// by a search of cu, 32 ways at a time, without a scan over the batch.  Lane i holds dimensions 4 i .. 4 i + 3 of all 16
 // tokens of both planes, so they are read once, in whole rows, with 8 KiB a warp
 // under way, and the maximum, the codes and the 4 x 4 byte transposes of V stay in
 // registers.  The sequence's first unit alone reads and writes its tail, each lane
@@ -232,18 +232,18 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 2) kv8_append_kernel(const 
             return w;
         w.h = (uint32_t)(item % a.num_kv_heads);
         const int64_t unit = (int64_t)(item / a.num_kv_heads);
-        uint32_t b = 0, n = a.num_seqs;  // the last b with cu[b] / 16 + 2 b <= unit, or 0
+        uint32_t b = 0, n = a.num_seqs;  // the last b with cu[b] / 16 + b <= unit, or 0
         while (n > 1) {
             const uint32_t step = (n + 31) / 32, at = b + step * (uint32_t)lane;
             const bool before =
-                step * (uint32_t)lane < n && (int64_t)(a.cu[at] >> 4) + 2 * (int64_t)at <= unit;
+                step * (uint32_t)lane < n && (int64_t)(a.cu[at] >> 4) + (int64_t)at <= unit;
             // cu may decrease in a bad call: then any b will do
             const int last = 31 - __clz(__ballot_sync(0xFFFFFFFFu, before) | 1u);
             n = min(step, n - step * (uint32_t)last);
             b += step * (uint32_t)last;
         }
         const int64_t c0 = a.cu[b], c1 = a.cu[b + 1], L0 = a.lens[b], L1 = L0 + (c1 - c0);
-        const int64_t j = unit - ((c0 >> 4) + 2 * (int64_t)b);
+        const int64_t j = unit - ((c0 >> 4) + (int64_t)b);
         if (j < 0 || c0 < 0 || c1 <= c0 || c1 > (int64_t)a.num_tokens)
             return w;
         if (L0 < 0 || (L1 >> 4) > (int64_t)a.max_pages) {
@@ -1273,12 +1273,12 @@ extern "C" int rt_kv8_append(const rt_kv8_append_params_t *p, const void *k, con
     a.num_kv_heads = p->num_kv_heads;
     a.num_tokens = p->num_tokens;
     a.max_pages = p->max_pages_per_seq;
-    const uint64_t units = (uint64_t)p->num_tokens / 16u + 2ull * p->num_seqs;
+    const uint64_t units = (uint64_t)p->num_tokens / 16u + p->num_seqs;
     a.n_items = units * p->num_kv_heads;
     uint64_t blocks = (a.n_items + kAppendWarps - 1) / kAppendWarps;
-    // Persistent warps hide the search behind the loads; a short call (mostly units
-    // without work) is over sooner with a warp to an item (256 sequences of one token:
-    // 6.0 against 8.1 us).
+    // Persistent warps hide the search behind the loads; a short call (many units with
+    // a tail's few tokens alone) is over sooner with a warp to an item (512 sequences
+    // of one token, 8 KV heads: 8.3 against 10.6 us).
     const uint64_t sms = (uint64_t)rt::num_sms();
     if (blocks > 6u * sms)
         blocks = 2u * sms;
