@@ -547,3 +547,34 @@ def test_padded_tokens_and_shared_pages(pkg, cuda):
     lens = [32, 56]
     q = torch.randn(2, 8, 128, generator=g, device=cuda).bfloat16()
     check(attend(pkg, cuda, q, *bufs, table, lens), q, *bufs, table, lens)
+
+
+@pytest.mark.parametrize("chunk", [0, 8])
+def test_captured_splits_replay(pkg, cuda, chunk):
+    """Split rows, captured in two graphs that replay in turn and at once on two streams, as
+    lengths and queries change between the replays."""
+    lens = [9000, 300, 5000, 17]
+    q, *rest, table = make(pkg, cuda, lens, 4, 4, "e4m3", seed=31)
+    td, ld = torch.from_numpy(table).to(cuda), torch.tensor(lens, dtype=torch.int32, device=cuda)
+    g = torch.Generator(device=cuda).manual_seed(32)
+    kw = dict(max_seq_len=9000, chunk_pages=chunk)
+    pkg.kv8_decode_attention(q, *rest, td, ld, **kw)
+    graphs, outs, streams = [], [], [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            outs.append([pkg.kv8_decode_attention(q, *rest, td, ld, **kw) for _ in range(2)])
+        graphs.append(graph)
+    for cut in (0, 1, 700, 16):
+        now = [max(n - cut, 0) for n in lens]
+        ld.copy_(torch.tensor(now, dtype=torch.int32))
+        q.copy_(torch.randn(q.shape, generator=g, device=cuda))
+        want = pkg.kv8_decode_attention(q, *rest, td, ld, **kw)
+        check(want, q, *rest, table, now)
+        torch.cuda.synchronize()
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, want) for pair in outs for o in pair)
