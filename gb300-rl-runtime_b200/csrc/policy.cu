@@ -19,8 +19,8 @@
 // The floor is the logits read once and the gradient written once, at the rate of a
 // copy (6,547 GB/s measured here).  fp32 is bound by that: 8,192 rows x 32,000 with
 // gradient and entropy 343 us, 93% of copy.  bf16 has two exponentials for every 4
-// bytes that move: 200 us, 80%, with the exponential unit 59% and the issue slots 56%
-// busy.  Small calls are bound by latency: 256 rows x 32,000 fp32 without gradient 8.0
+// bytes that move: 200 us, 80%, with the exponential unit 59% and the issue slots 60%
+// busy (a quarter of the exponentials as polynomials on the multiply-add pipes: 220).  Small calls are bound by latency: 256 rows x 32,000 fp32 without gradient 8.0
 // us (floor 5.0), 64 rows with gradient 8.0 us (floor 2.5).
 #include <cfloat>
 #include <cmath>
