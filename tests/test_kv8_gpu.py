@@ -578,3 +578,27 @@ def test_captured_splits_replay(pkg, cuda, chunk):
                 graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(o, want) for pair in outs for o in pair)
+
+
+@pytest.mark.parametrize("start", [1, 15, 16, 40])
+def test_append_of_tokens_from_the_middle(pkg, cuda, start):
+    """cu_tokens that begin and end inside the rows, and a batch of many empty sequences."""
+    g = torch.Generator(device=cuda).manual_seed(start)
+    new = [0] * 40 + [31, 0, 1, 16] + [0] * 40 + [50]
+    old = [(7 * i) % 33 for i in range(len(new))]
+    T = start + sum(new) + 9
+    k, v = torch.randn(2, T, 2, 128, generator=g, device=cuda).bfloat16()
+    n_pages = sum((a + b) // 16 for a, b in zip(old, new)) + 2
+    bufs = cache(pkg, cuda, "s8", n_pages, len(new), 2, 6)
+    table = tables([a + b for a, b in zip(old, new)], n_pages, 7)
+    model = Model(*bufs, "s8")
+    error = torch.zeros(1, dtype=torch.int32, device=cuda)
+    cu = np.concatenate([[start], start + np.cumsum(new)]).astype(np.int32)
+    pkg.kv8_append(k, v, torch.from_numpy(cu).to(cuda),
+                   torch.tensor(old, dtype=torch.int32, device=cuda),
+                   torch.from_numpy(table).to(cuda), *bufs, error=error)
+    rows = np.stack([bf16(k), bf16(v)], 2)
+    for b, n in enumerate(new):
+        model.append(b, old[b], rows[cu[b]:cu[b] + n], table[b])
+    model.check(*bufs)
+    assert error.item() == 0
