@@ -823,9 +823,12 @@ __global__ void __launch_bounds__(512) policy_stats_kernel(const rt_policy_row_t
     }
 }
 
-// Short rows, when there are enough of them for all SMs' warps, are a warp's own.
+// Short rows are a warp's own, those above 1,000 once there are more than CTAs for
+// them at once (loss with gradient: 300 rows of 500 fp32 6.3 us, a CTA each 7.9; 8,192
+// of 4,000 bf16 38 against 59; 592 of 4,000 fp32 10.3 against 9.3).
 // Else CTAs to a row: as few as make a slice fit the target, then more while the
-// rows would leave SMs idle and a slice keeps 8 KiB.  A group (a cluster or a warp)
+// rows would leave SMs idle and a slice keeps 8 KiB (16 rows of 32,000 bf16: 7.1 us,
+// one CTA a row 10.0).  A group (a cluster or a warp)
 // that takes several rows starts each row's copy as its warps end their parts of the
 // row before.  Equal shares, all groups at once, where no group waits long for the
 // last (4,096 rows of 8,000 fp32, 6.9 turns: 50 us, one row to a group 62); else one
@@ -882,7 +885,7 @@ template <typename T, Mode MODE>
 int launch_shape(RowArgs &a, cudaStream_t stream, const char *what)
 {
     const uint64_t row = (uint64_t)a.vocab * sizeof(T) + 16u, sms = (uint64_t)rt::num_sms();
-    if (a.vocab <= 6000u && a.num_rows >= 4u * sms)
+    if (a.vocab <= 1000u || (a.vocab <= 6000u && a.num_rows > kCtasPerSm * sms))
         return launch_rows<T, MODE, true>(a, 1u, stream, what);
     uint32_t k = 1;
     while (k < kMaxCluster && row > (uint64_t)k * kSmemTarget)
