@@ -592,8 +592,9 @@ def kv8_append(k, v, cu_tokens, seq_lens, page_table, pages, scales, tail, error
 def kv8_decode_attention(q, pages, scales, tail, page_table, seq_lens, max_seq_len, scale=None,
                          out=None, chunk_pages=0, workspace=None, error=None, stream=None):
     """rt_kv8_decode_attention: q bf16 [B, Hq, 128] over the cache of kv8_append; returns
-    fp32 [B, Hq, 128].  max_seq_len bounds every seq_lens[b].  workspace: uint8, by default
-    a new one (from torch's allocator, on the current stream)."""
+    fp32 [B, Hq, 128].  max_seq_len bounds every seq_lens[b]; it may be larger than what P
+    pages and a tail hold, and then it is that.  workspace: uint8, by default a new one (from
+    torch's allocator, on the current stream)."""
     if _torch is None:
         _tm()
     B = seq_lens.shape[0]
@@ -611,7 +612,7 @@ def kv8_decode_attention(q, pages, scales, tail, page_table, seq_lens, max_seq_l
     P = _width(page_table)
     if not (0 <= max_seq_len <= 0x7FFFFFFF and 0 <= chunk_pages <= 128):
         raise ValueError("max_seq_len 0 .. 2^31 - 1, chunk_pages 0 .. 128")
-    p = rt_kv8_attn_params_t(B, Hq, h, P, max_seq_len, fmt, n_pages,
+    p = rt_kv8_attn_params_t(B, Hq, h, P, min(max_seq_len, 16 * P + 15), fmt, n_pages,
                              q_stride if B > 1 else Hq * 128,
                              128 ** -0.5 if scale is None else scale, chunk_pages)
     ref = ctypes.byref(p)

@@ -233,7 +233,9 @@ typedef struct {
     uint32_t num_q_heads;        /* a multiple of num_kv_heads, 1 to 8 to a KV head */
     uint32_t num_kv_heads;
     uint32_t max_pages_per_seq;  /* page-table row stride */
-    uint32_t max_seq_len;        /* upper bound on every seq_lens[b] */
+    uint32_t max_seq_len;        /* upper bound on every seq_lens[b]; at most
+                                    16 * max_pages_per_seq + 15, what the pages and a tail
+                                    hold (more is RT_EINVAL; the binding lowers it) */
     uint32_t format;             /* RT_KV8_* */
     uint64_t arena_pages;
     uint64_t q_stride;           /* elements between sequences' queries, >= num_q_heads * 128
