@@ -409,10 +409,8 @@ def run(state):
                       s["scales"], s["tail"])
         return {"pages": s["pages"], "scales": s["scales"], "tail": s["tail"]}
     if c["op"] == "attention":
-        # no sequence is longer than the case's bound, nor than its page table and a tail
-        most = min(c["len_max"], (s["page_table"].shape[1] + 1) * PAGE - 1)
         return rt.kv8_decode_attention(s["q"], s["pages"], s["scales"], s["tail"],
-                                       s["page_table"], s["seq_lens"], max_seq_len=most)
+                                       s["page_table"], s["seq_lens"], max_seq_len=c["len_max"])
     if c["op"] == "logprobs":
         if c["backward"]:
             return rt.token_logprobs_backward(s["logits"], s["tokens"], s["dlogprobs"],
