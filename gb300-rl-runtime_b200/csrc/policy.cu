@@ -437,7 +437,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) row_kernel(const RowArgs
             T *out = dst - r.skip;
             for (uint32_t v = r.from + lane * N; v < r.to; v += 32 * N)
                 *reinterpret_cast<uint4 *>(out + v) = make_uint4(0u, 0u, 0u, 0u);
-            for (uint32_t v = max(r.lo, r.skip) + lane; v < r.from; v += 32)
+            // a row may end inside its first vector
+            for (uint32_t v = max(r.lo, r.skip) + lane; v < min(r.from, r.end); v += 32)
                 out[v] = from_float<T>(0.0f);
             for (uint32_t v = r.to + lane; v < min(r.hi, r.end); v += 32)
                 out[v] = from_float<T>(0.0f);
