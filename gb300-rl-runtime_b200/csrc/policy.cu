@@ -612,11 +612,21 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) row_kernel(const RowArgs
                 const float A = __shfl_sync(0xFFFFFFFFu, adv, i), w = __shfl_sync(0xFFFFFFFFu, weight, i);
                 const float before = __shfl_sync(0xFFFFFFFFu, old_lp, i);
                 const float ref = __shfl_sync(0xFFFFFFFFu, ref_lp, i);
-                const float ratio = a.old_lp ? expf((float)(lp - (double)before)) : 1.0f;
+                const float apart = a.old_lp ? (float)(lp - (double)before) : 0.0f;
+                const float ratio = a.old_lp ? expf(apart) : 1.0f;
                 const float held = fminf(fmaxf(ratio, 1.0f - a.clip_low), 1.0f + a.clip_high);
-                const bool clipped = ratio * A > held * A;
-                const float policy = clipped ? -held * A : -ratio * A;
-                float kl = 0.0f, slope = clipped ? 0.0f : -ratio * A;
+                // Where the ratio, or its product, leaves fp32, products of its root stay: an
+                // advantage of 0 gives 0, and a weight may bring the slope back.
+                float gain = ratio * A, pull = 0.0f;
+                const bool large = !(fabsf(gain) < 0x1p100f) && apart == apart;
+                if (large) {
+                    const float half = expf(0.5f * apart), Aw = A * w;
+                    gain = A == 0.0f ? 0.0f : half * (half * A);
+                    pull = Aw == 0.0f ? 0.0f : half * (half * Aw);
+                }
+                const bool clipped = gain > held * A;
+                const float policy = clipped ? -held * A : -gain;
+                float kl = 0.0f, slope = clipped || large ? 0.0f : -gain;
                 if (a.kl_coef != 0.0f) {
                     const float gap = (float)((double)ref - lp), x = expm1f(gap);
                     // e^g - 1 - g; by its series where the subtraction would lose digits
@@ -628,7 +638,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) row_kernel(const RowArgs
                     slope -= a.kl_coef * x;
                 }
                 const float loss = policy + a.kl_coef * kl - a.entropy_coef * ent;
-                g_lp = slope * w;
+                g_lp = slope * w - (clipped ? 0.0f : pull);
                 g_h = -a.entropy_coef * w;
                 if (first && lane == 0) {
                     float4 *to = reinterpret_cast<float4 *>(a.rows + row);

@@ -1,10 +1,12 @@
 """The row operators over wide ranges: rows shorter than a vector, large ratios, the longest
 rows that a warp takes alone.  References and tolerances are those of test_policy_gpu.py,
 except where a test states its own."""
+import math
+
 import pytest
 import torch
 
-from test_policy_gpu import case, grad64, logits_of, policy64, rows64
+from test_policy_gpu import E, case, grad64, logits_of, policy64, rows64
 
 pytestmark = pytest.mark.gpu
 
@@ -53,3 +55,44 @@ def test_rows_without_gradient_stay_inside(pkg, cuda, dtype, V, extra):
                 assert bool((flat[~inside] == 5).all())
                 assert bool((view[off] == 0).all())
                 assert bool(((view[~off].double() - want[~off]).abs() <= bound[~off]).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [50, 5000])
+def test_policy_of_large_ratios(pkg, cuda, dtype, V):
+    """Log-probabilities far above the old ones: e^gap leaves fp32 at 88.7, its product with an
+    advantage of 0 is 0, and with a small one a number.  The product is off by the share that
+    its exponent is (lp's error, and half a step of a gap below 256: 2^-17), and by that of two
+    exponentials and two products, at most 2^-21 each."""
+    gaps = [0.0, 50.0, 88.0, 89.0, 95.0, 120.0, 170.0, 200.0]
+    values = [0.0, 1e-30, -1e-30, -1e-3, 1.0, -1.0]
+    R = len(gaps) * len(values)
+    logits, tokens = logits_of(cuda, R, V, dtype, 71)
+    gap = torch.tensor(gaps, dtype=torch.float64, device=cuda).repeat_interleave(len(values))
+    adv = torch.tensor(values, device=cuda).repeat(len(gaps))
+    p, logp, d, lp, h, _ = rows64(logits, tokens, 1.0)
+    old = (lp - gap).float()
+    w = torch.full((R,), 0.5, device=cuda)
+    r = pkg.policy_loss(logits, tokens, w, adv, old)
+    ratio = (lp - old.double()).exp()
+    a = adv.double()
+    cut = ratio * a > ratio.clip(0.8, 1.2) * a
+    want = -torch.where(cut, ratio.clip(0.8, 1.2) * a, ratio * a)
+    share = E + 2.0 ** -24 * lp.abs() + 2.0 ** -17 + 4 * 2.0 ** -21
+    big = torch.finfo(torch.float32).max
+    fits = want.abs() < big
+    near = (r.row_loss.double() - want).abs() <= share * want.abs()
+    assert bool((near | ~fits).all()) and bool((r.row_loss[~fits] == math.inf).all())
+    assert bool((r.policy == r.row_loss).all())
+    assert torch.equal(r.clipped.bool(), cut)
+    # a slope beyond fp32 has no gradient in numbers
+    slope = torch.where(cut, 0.0, -ratio * a) * 0.5
+    ok = slope.abs() < big
+    zero = torch.zeros_like(slope)
+    ref, tol = grad64(p, logp, d, h, tokens, torch.where(ok, slope, 0.0), zero, 1.0, dtype)
+    hit = torch.zeros_like(ref).scatter_(1, tokens.long()[:, None], 1.0)
+    tol = tol + (share * slope.abs())[:, None] * (p + hit)
+    assert bool(((r.dlogits[ok].double() - ref[ok]).abs() <= tol[ok]).all())
+    assert bool((r.dlogits[adv == 0] == 0).all())
+    none = pkg.policy_loss(logits, tokens, w, torch.zeros_like(adv), old)
+    assert bool((none.stats[:2] == 0).all()) and bool((none.dlogits == 0).all())
