@@ -626,7 +626,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) row_kernel(const RowArgs
                 }
                 const bool clipped = gain > held * A;
                 const float policy = clipped ? -held * A : -gain;
-                float kl = 0.0f, slope = clipped || large ? 0.0f : -gain;
+                float kl = 0.0f, penalty = 0.0f, slope = clipped || large ? 0.0f : -gain;
+                if (clipped)
+                    pull = 0.0f;
                 if (a.kl_coef != 0.0f) {
                     const float gap = (float)((double)ref - lp), x = expm1f(gap);
                     // e^g - 1 - g; by its series where the subtraction would lose digits
@@ -635,10 +637,17 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) row_kernel(const RowArgs
                         kl = gap * gap *
                              (0.5f + gap * (1.f / 6 + gap * (1.f / 24 + gap * (1.f / 120 +
                               gap * (1.f / 720 + gap * (1.f / 5040 + gap * (1.f / 40320)))))));
-                    slope -= a.kl_coef * x;
+                    penalty = a.kl_coef * kl;
+                    if (gap > 80.0f) {  // as above
+                        const float half = expf(0.5f * gap);
+                        penalty = half * (half * a.kl_coef) - a.kl_coef * (gap + 1.0f);
+                        pull += half * (half * (a.kl_coef * w));
+                    } else {
+                        slope -= a.kl_coef * x;
+                    }
                 }
-                const float loss = policy + a.kl_coef * kl - a.entropy_coef * ent;
-                g_lp = slope * w - (clipped ? 0.0f : pull);
+                const float loss = policy + penalty - a.entropy_coef * ent;
+                g_lp = slope * w - pull;
                 g_h = -a.entropy_coef * w;
                 if (first && lane == 0) {
                     float4 *to = reinterpret_cast<float4 *>(a.rows + row);

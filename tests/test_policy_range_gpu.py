@@ -96,3 +96,42 @@ def test_policy_of_large_ratios(pkg, cuda, dtype, V):
     assert bool((r.dlogits[adv == 0] == 0).all())
     none = pkg.policy_loss(logits, tokens, w, torch.zeros_like(adv), old)
     assert bool((none.stats[:2] == 0).all()) and bool((none.dlogits == 0).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [50, 5000])
+def test_policy_of_large_divergences(pkg, cuda, dtype, V):
+    """Reference log-probabilities far above: e^gap leaves fp32 at 88.7, its products with the
+    coefficient and the weight later.  Off by the shares that the test above counts."""
+    gaps = [79.0, 81.0, 88.0, 89.5, 91.0, 100.0, 120.0]
+    weights = [1e-3, 1e-7, 1e-12, 1e-20]
+    coef = 1e-2
+    R = len(gaps) * len(weights)
+    logits, tokens = logits_of(cuda, R, V, dtype, 72)
+    logits[::3, 1] = -math.inf
+    tokens[::3] = torch.where(tokens[::3] == 1, 2, tokens[::3])
+    gap = torch.tensor(gaps, dtype=torch.float64, device=cuda).repeat_interleave(len(weights))
+    w = torch.tensor(weights, device=cuda).repeat(len(gaps))
+    p, logp, d, lp, h, _ = rows64(logits, tokens, 1.0)
+    ref_lp = (lp + gap).float()
+    adv = torch.linspace(-1, 1, R, device=cuda)
+    r = pkg.policy_loss(logits, tokens, w, adv, None, ref_lp, kl_coef=coef)
+    apart = ref_lp.double() - lp
+    share = E + 2.0 ** -24 * lp.abs() + 2.0 ** -17 + 4 * 2.0 ** -21
+    big = torch.finfo(torch.float32).max
+
+    def same(got, want):
+        fits = want < big * 0.99
+        near = (got.double() - want).abs() <= share * want.abs()
+        assert bool((near | ~fits).all()) and bool((got[want > big * 1.01] == math.inf).all())
+
+    same(r.kl, apart.exp() - apart - 1)
+    same(r.row_loss, coef * (apart.exp() - apart - 1) - adv.double())
+    slope = (coef * (1 - apart.exp()) - adv.double()) * w.double()
+    ok = slope.abs() < big * 0.99
+    assert int(ok.sum()) > R // 2
+    zero = torch.zeros_like(slope)
+    ref, tol = grad64(p, logp, d, h, tokens, torch.where(ok, slope, 0.0), zero, 1.0, dtype)
+    hit = torch.zeros_like(ref).scatter_(1, tokens.long()[:, None], 1.0)
+    tol = tol + (share * slope.abs())[:, None] * (p + hit)
+    assert bool(((r.dlogits[ok].double() - ref[ok]).abs() <= tol[ok]).all())
