@@ -560,7 +560,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) row_kernel(const RowArgs
                            make_uint4((uint32_t)st.R, __float_as_uint(st.s), __float_as_uint(st.u),
                                       __float_as_uint(l_hit)));
             if (warp == 0) {
-                if (!rt::mbar_wait_bounded(bar, exchanges >> 1 & 1u, kWaitLimitNs)) {
+                if (!rt::mbar_wait_bounded<true>(bar, exchanges >> 1 & 1u, kWaitLimitNs)) {
                     late = true;
                     if (a.error)
                         atomicCAS(a.error, 0, kErrTimeout);

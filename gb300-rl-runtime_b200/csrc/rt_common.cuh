@@ -57,6 +57,20 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity)
     return ok != 0u;
 }
 
+// The same where other CTAs of the cluster have written what the phase stands for.
+__device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t parity)
+{
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0u;
+}
+
 // Non-blocking probe of a phase (test_wait never suspends the thread, unlike
 // try_wait): for a producer polling several barriers.
 __device__ __forceinline__ bool mbar_test_wait(uint32_t bar, uint32_t parity)
@@ -74,13 +88,17 @@ __device__ __forceinline__ bool mbar_test_wait(uint32_t bar, uint32_t parity)
 
 // Wait for the phase of `bar` with the given parity; gives up after
 // `limit_ns` of wall time and returns false (the caller reports an error
-// instead of hanging the GPU).
+// instead of hanging the GPU).  CLUSTER: what it waits for comes from other CTAs.
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool mbar_wait_bounded(uint32_t bar, uint32_t parity, uint64_t limit_ns)
 {
-    if (mbar_try_wait(bar, parity))
+    auto try_wait = [&]() {
+        return CLUSTER ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity);
+    };
+    if (try_wait())
         return true;
     const uint64_t t0 = globaltimer_ns();
-    while (!mbar_try_wait(bar, parity)) {
+    while (!try_wait()) {
         if (globaltimer_ns() - t0 > limit_ns)
             return false;
     }
