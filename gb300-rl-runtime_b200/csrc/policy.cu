@@ -104,12 +104,15 @@ __device__ __forceinline__ uint32_t cluster_rank()
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
     return r;
 }
+// Aligned: all lanes of a warp execute them together.
 __device__ __forceinline__ void cluster_arrive()
 {
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void cluster_wait()
 {
+    __syncwarp();
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // Store to the shared memory of the cluster's CTA `rank`, at the addresses that
@@ -832,7 +835,6 @@ __global__ void __launch_bounds__(512) policy_stats_kernel(const rt_policy_row_t
                      : "=r"(to) : "r"(rt::smem_u32(&shares[rank][threadIdx.x])));
         asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(to), "d"(s) : "memory");
     }
-    __syncwarp();
     cluster_arrive();
     cluster_wait();
     if (rank == 0 && threadIdx.x < 5) {
