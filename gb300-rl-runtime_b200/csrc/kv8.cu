@@ -404,7 +404,7 @@ struct AttnArgs {
     const __nv_bfloat16 *tail;
     const int32_t *page_table, *lens;
     float *out;
-    float *part_o;    // [num_seqs][num_kv_heads][max_chunks][G][128], unnormalised
+    float *part_o;    // [num_seqs][num_kv_heads][max_chunks][G][128], each chunk's own mean
     float2 *part_ml;  // [num_seqs][num_kv_heads][max_chunks][G] (maximum, sum), base 2
     int32_t *error;
     uint64_t q_stride, arena_pages;
@@ -502,10 +502,9 @@ struct Softmax {
 
 __device__ __forceinline__ float exp2i(int e) { return __int_as_float((127 + e) << 23); }
 
-// Bring O to a unit that holds V scales of up to `top` (bits of a float, no sign).
-__device__ __forceinline__ void raise_unit(Softmax &st, uint32_t top)
+// Bring O to a unit of 2^(v - 14) where it is below.
+__device__ __forceinline__ void raise_unit(Softmax &st, int v)
 {
-    const int v = min((int)(top >> 23) - 126, 127);
     if (v > st.v) {
         // from -110 the step can be 237: in two factors
         const float f = exp2i(max(st.v - v, -126)), f2 = exp2i(min(0, st.v - v + 126));
@@ -517,6 +516,8 @@ __device__ __forceinline__ void raise_unit(Softmax &st, uint32_t top)
                 st.o[i][u] = st.o[i][u] * f * f2;
     }
 }
+// The exponent above a V scale (bits of a float, no sign).
+__device__ __forceinline__ int unit_of(uint32_t scale) { return min((int)(scale >> 23) - 126, 127); }
 
 // New maxima for the scores of NP times 16 tokens (rows g and g + 8); s becomes
 // exp2(s - m), and what was summed before is brought to the new maxima.  A warp
@@ -769,7 +770,7 @@ __device__ __forceinline__ void pages_step(Softmax &st, const uint4 *(&blk)[NP],
     uint32_t top = __float_as_uint(sv[0]) & 0x7FFFFFFFu;
     if constexpr (NP > 1)
         top = max(top, __float_as_uint(sv[1]) & 0x7FFFFFFFu);
-    raise_unit(st, top);
+    raise_unit(st, unit_of(top));
     const bool low_half = DUP && (threadIdx.x & 2) != 0;  // columns 4..7
 #pragma unroll
     for (int p = 0; p < NP; p++) {
@@ -811,6 +812,10 @@ __device__ __forceinline__ void pages_step(Softmax &st, const uint4 *(&blk)[NP],
 // same products on bf16 fragments, P in three bf16 terms (24 bits).  Rows past
 // the tail's end hold anything: their scores are -inf and their V bits cleared.
 // With DUP the first four columns carry all three terms.
+//
+// V has bf16's range: P is at most 2^-5, so that 16 products stay in fp32's, and they
+// are summed apart, for O's unit may be so large that P in it would lose digits; with
+// a unit of at least 2^6 O holds their sum.
 template <bool DUP>
 __device__ __forceinline__ void tail_step(Softmax &st, const uint8_t *tk, const uint8_t *tv,
                                           const __nv_bfloat16 *q_row, bool has_q, uint32_t n_tail,
@@ -834,8 +839,9 @@ __device__ __forceinline__ void tail_step(Softmax &st, const uint8_t *tk, const 
     x[0][3] = in1 ? x[0][3] * scale_log2 : -INFINITY;
     softmax_step<1>(st, x);
     uint32_t p[3][2];
-    raise_unit(st, 0x3F800000u);
-    const float unit = DUP && (threadIdx.x & 2) ? 0.0f : exp2i(14 - st.v);
+    raise_unit(st, 20);
+    const float unit = DUP && (threadIdx.x & 2) ? 0.0f : 0x1p-5f;
+    const float back = exp2i(19 - st.v);
 #pragma unroll
     for (int u = 0; u < 4; u++)
         x[0][u] *= unit;
@@ -863,9 +869,13 @@ __device__ __forceinline__ void tail_step(Softmax &st, const uint8_t *tk, const 
         const uint32_t d0 = 16 * i + g;
         const uint32_t f[4] = {pair(2 * c, d0) & keep0, pair(2 * c, d0 + 8) & keep0,
                                pair(2 * c + 8, d0) & keep1, pair(2 * c + 8, d0 + 8) & keep1};
+        float d[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < 3; k++)
-            rt::mma_bf16_16816(st.o[i], f, p[k][0], p[k][1]);
+            rt::mma_bf16_16816(d, f, p[k][0], p[k][1]);
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+            st.o[i][u] = fmaf(d[u], back, st.o[i][u]);
     }
 }
 
@@ -1025,37 +1035,42 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) kv8_decode_kernel(con
     }
     __syncthreads();  // all slots have been read
     float *merge = reinterpret_cast<float *>(smem);
+    // Divided by the sum here: a mean of V is in fp32's range where a sum may not be.
+    const uint64_t row = (uint64_t)b * H + h, slot = row * a.max_chunks + chunk;
     {
         const float unit = exp2i(st.v - 14);
         // all maxima -infinity: no page was read, or all scores were NaN
-        auto weight = [&](int col) {
-            float M = -INFINITY;
+        auto weight = [&](uint32_t col) {
+            float M = -INFINITY, l = 0.0f, own = 0.0f;
 #pragma unroll
             for (int w = 0; w < kWarps; w++)
                 M = fmaxf(M, ml[w][col].x);
-            return M == -INFINITY ? unit : rt::fast_exp2(ml[warp][col].x - M) * unit;
+#pragma unroll
+            for (int w = 0; w < kWarps; w++) {
+                const float x = M == -INFINITY ? 1.0f : rt::fast_exp2(ml[w][col].x - M);
+                l = fmaf(ml[w][col].y, x, l);
+                own = w == warp ? x : own;
+            }
+            if (n_chunks > 1 && warp == 0 && g == 0 && col < G)
+                a.part_ml[slot * G + col] = make_float2(M, l);
+            return l == 0.0f ? 0.0f : __fdividef(own, l);
         };
         const float w0 = weight(2 * c), w1 = weight(2 * c + 1);
         float *to = merge + ((size_t)warp * 8 + 2 * c) * kHeadPitch + g;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            to[16 * i] = st.o[i][0] * w0;
-            to[16 * i + kHeadPitch] = st.o[i][1] * w1;
-            to[16 * i + 8] = st.o[i][2] * w0;
-            to[16 * i + 8 + kHeadPitch] = st.o[i][3] * w1;
+            to[16 * i] = st.o[i][0] * w0 * unit;
+            to[16 * i + kHeadPitch] = st.o[i][1] * w1 * unit;
+            to[16 * i + 8] = st.o[i][2] * w0 * unit;
+            to[16 * i + 8 + kHeadPitch] = st.o[i][3] * w1 * unit;
         }
     }
     __syncthreads();
-    const uint64_t row = (uint64_t)b * H + h, slot = row * a.max_chunks + chunk;
+    float *means = n_chunks == 1 ? a.out + row * G * 128u : a.part_o + slot * G * 128u;
     for (uint32_t r = warp; r < G; r += kWarps) {  // a warp to a head, four dimensions a lane
-        float M = -INFINITY, l = 0.0f;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < kWarps; w++)
-            M = fmaxf(M, ml[w][r].x);
-#pragma unroll
         for (int w = 0; w < kWarps; w++) {
-            l += ml[w][r].y * (M == -INFINITY ? 1.0f : rt::fast_exp2(ml[w][r].x - M));
 #pragma unroll
             for (uint32_t col = r; col < 8u; col += DUP ? 4u : 8u) {
                 const float4 o = *reinterpret_cast<const float4 *>(merge + (w * 8 + col) * kHeadPitch + 4 * lane);
@@ -1065,15 +1080,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) kv8_decode_kernel(con
                 acc.w += o.w;
             }
         }
-        if (n_chunks == 1) {
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            reinterpret_cast<float4 *>(a.out + (row * G + r) * 128u)[lane] =
-                make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
-        } else {
-            reinterpret_cast<float4 *>(a.part_o + (slot * G + r) * 128u)[lane] = acc;
-            if (lane == 0)
-                a.part_ml[slot * G + r] = make_float2(M, l);
-        }
+        reinterpret_cast<float4 *>(means + r * 128u)[lane] = acc;
     }
 }
 
@@ -1125,44 +1132,52 @@ __global__ void __launch_bounds__(WARPS == 1 ? 256 : WARPS * 32) kv8_merge_kerne
 #pragma unroll
         for (int u = 0; u < U; u++)
             top = fmaxf(top, s[u].x);
-        const float w0 = weight(m, top);
+        // weights that sum to 1, so that acc stays a mean
+        float w0 = l * weight(m, top), wt[U];
+        l = w0;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            wt[u] = s[u].y * weight(s[u].x, top);
+            l += wt[u];
+        }
+        const float inv = l == 0.0f ? 0.0f : __fdividef(1.0f, l);
         m = top;
-        l *= w0;
+        w0 *= inv;
         acc.x *= w0;
         acc.y *= w0;
         acc.z *= w0;
         acc.w *= w0;
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const float wt = weight(s[u].x, top);
-            l += s[u].y * wt;
-            acc.x += o[u].x * wt;
-            acc.y += o[u].y * wt;
-            acc.z += o[u].z * wt;
-            acc.w += o[u].w * wt;
+            wt[u] *= inv;
+            acc.x += o[u].x * wt[u];
+            acc.y += o[u].y * wt[u];
+            acc.z += o[u].z * wt[u];
+            acc.w += o[u].w * wt[u];
         }
     }
     if constexpr (WARPS == 1) {
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        reinterpret_cast<float4 *>(a.out + item * 128u)[lane] =
-            make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+        reinterpret_cast<float4 *>(a.out + item * 128u)[lane] = acc;
     } else {
         warp_o[warp][lane] = acc;
         if (lane == 0)
             warp_ml[warp] = make_float2(m, l);
         __syncthreads();
         if (threadIdx.x < 128) {
-            float top = -INFINITY, sum = 0.0f, den = 0.0f;
+            float top = -INFINITY, sum = 0.0f, den = 0.0f, wt[WARPS];
 #pragma unroll
             for (int w = 0; w < WARPS; w++)
                 top = fmaxf(top, warp_ml[w].x);
 #pragma unroll
             for (int w = 0; w < WARPS; w++) {
-                const float wt = weight(warp_ml[w].x, top);
-                sum += reinterpret_cast<const float *>(warp_o[w])[threadIdx.x] * wt;
-                den += warp_ml[w].y * wt;
+                wt[w] = warp_ml[w].y * weight(warp_ml[w].x, top);
+                den += wt[w];
             }
-            a.out[item * 128u + threadIdx.x] = den == 0.0f ? 0.0f : sum / den;
+            const float inv = den == 0.0f ? 0.0f : __fdividef(1.0f, den);
+#pragma unroll
+            for (int w = 0; w < WARPS; w++)
+                sum += reinterpret_cast<const float *>(warp_o[w])[threadIdx.x] * (wt[w] * inv);
+            a.out[item * 128u + threadIdx.x] = sum;
         }
     }
 }
