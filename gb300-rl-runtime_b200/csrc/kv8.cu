@@ -564,31 +564,34 @@ __device__ __forceinline__ void softmax_step(Softmax &st, float (&s)[NP][4])
 }
 
 // The query in the codes' own format.  With an element q scaled by a power of
-// two, s8 writes the integer nearest to it in digits of base 256, each in [-128,
-// 127]; e4m3 writes it as a sum of terms t_i 2^-4i, each the nearest to 16 times
-// what the ones before have left.  Products with codes are exact and their sums
-// kept in fp32 or integers, so K needs no conversion: a word of it is an operand
-// as it lies.
+// two, s8 writes it as an integer in digits of base 256, each in [-128, 127]; e4m3
+// as a sum of terms t_i 2^-4i, each the nearest to 16 times what the ones before have
+// left.  Products with codes are exact and their sums kept in fp32 or integers, so K
+// needs no conversion: a word of it is an operand as it lies.
 //
 // Up to 4 heads to a KV head (DUP): 4 digits, the 8 columns of one product taking
 // two of them (columns 0..3 the one, 4..7 the other) and a second product the
-// other two.  More heads: 3 digits in 3 products.  What is lost of an element is
-// below 2^-30 (2^-22 with 3 digits of s8, 2^-26 with 3 of e4m3) of the row's
-// largest.  bf16's 8 bits fill two terms of e4m3 unless an element is below 2^-13
-// of the largest, so most rows need no more (`deep` is false).
+// other two.  More heads: a product to a digit, 4 of s8 and 3 of e4m3.  The digits
+// hold bf16's 8 bits down to elements 2^-22 (s8), 2^-21 (e4m3, 4 terms) or 2^-17 (3)
+// of the row's largest.  What the last product adds is 0 unless an element is below
+// 2^-14 (s8, more heads) or 2^-13 (e4m3), so most rows skip it (`deep` is false).  Rows
+// with elements that the digits do not hold take wide_step (`exact` is false): K may be
+// 0 where they are large, and then their score is what the small elements say.
 template <uint32_t FMT, bool DUP>
 struct Query {
-    static constexpr int kDigits = DUP ? 4 : 3, kProducts = DUP ? 2 : 3;
+    static constexpr int kDigits = DUP || FMT == RT_KV8_S8 ? 4 : 3, kProducts = DUP ? 2 : kDigits;
+    static constexpr bool kSkips = FMT == RT_KV8_E4M3 || !DUP;  // the last product is `deep`'s
+    // The row's largest element is brought to [2^kTop, 2^(kTop + 1)): a first digit of up
+    // to 63 (s8, with room for the carry) or 256 (e4m3).
+    static constexpr int kTop = FMT == RT_KV8_E4M3 ? 7 : 29;
     uint32_t f[kProducts][4][2];
     float k0, k1;  // factors of the scores of the lane's columns 2c and 2c + 1
-    bool deep;     // e4m3: digits past the second are not all 0 (the same in all lanes)
+    bool deep, exact;  // the same in all lanes
 
-    // Lane (g, c) holds, of column g, dimensions 16 s + 4 c .. + 3 for s = 0..7, as
-    // K's words hold them.
-    __device__ __forceinline__ void load(const __nv_bfloat16 *row, bool has, float scale_log2)
+    // Row g's elements of the lane, and the bits of the row's largest.
+    static __device__ __forceinline__ uint32_t fetch(const __nv_bfloat16 *row, bool has, uint2 (&qv)[8])
     {
-        const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-        uint2 qv[8];
+        const int c = threadIdx.x & 3;
 #pragma unroll
         for (int s = 0; s < 8; s++)
             qv[s] = has ? *reinterpret_cast<const uint2 *>(row + 16 * s + 4 * c) : make_uint2(0u, 0u);
@@ -598,11 +601,21 @@ struct Query {
             top2 = __vmaxu2(top2, __vmaxu2(qv[s].x & 0x7FFF7FFFu, qv[s].y & 0x7FFF7FFFu));
         uint32_t top = max(top2 & 0xFFFFu, top2 >> 16);
         top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-        top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-        // The row times 2^(kTop - e), its largest element in [2^kTop, 2^(kTop + 1)): a
-        // first digit of up to 127 (s8, with room for the carry) or 256 (e4m3).
-        constexpr int kTop = FMT == RT_KV8_E4M3 ? 7 : 8 * kDigits - 3;
-        const int e = min(max((int)(top >> 7) - 127, kTop - 126), 127);
+        return max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+    }
+    static __device__ __forceinline__ int exponent(uint32_t top)
+    {
+        return min(max((int)(top >> 7) - 127, kTop - 126), 127);
+    }
+
+    // Lane (g, c) holds, of column g, dimensions 16 s + 4 c .. + 3 for s = 0..7, as
+    // K's words hold them.
+    __device__ __forceinline__ void load(const __nv_bfloat16 *row, bool has, float scale_log2)
+    {
+        const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+        uint2 qv[8];
+        const uint32_t top = fetch(row, has, qv);
+        const int e = exponent(top);
         const float up = exp2i(kTop - e);
         // a row with a NaN or an infinity has no digits: its scores become NaN
         const float down = top >= 0x7F80u ? __int_as_float(0x7FC00000) : exp2i(e - kTop);
@@ -610,7 +623,7 @@ struct Query {
             const uint32_t w = u & 2 ? qv[s].y : qv[s].x;
             return __uint_as_float(u & 1 ? w & 0xFFFF0000u : w << 16) * up;
         };
-        deep = true;
+        bool left = false;  // something that the digits do not hold
         if constexpr (FMT == RT_KV8_E4M3) {
             // the first term cut off after 4 bits, the second has the other 4
             bool small = false;
@@ -660,6 +673,7 @@ struct Query {
                                 y = (y - v.y) * 16.0f;
                                 d[i] |= t << (8 * u);
                             }
+                            left |= x != 0.0f || y != 0.0f;
                         }
 #pragma unroll
                         for (int i = 0; i < kProducts; i++) {
@@ -674,25 +688,35 @@ struct Query {
             }
         } else {
             // A byte plus 128, carried on, less 128 is a digit: all of them at once.
-            constexpr uint32_t kBias = DUP ? 0x00808080u : 0x00008080u;
+            constexpr uint32_t kBias = 0x00808080u;
             // bytes of the first and second product's digits, as selectors
-            const uint32_t s0 = DUP ? (g < 4 ? 0x73u : 0x62u) : 0x62u;
-            const uint32_t s1 = DUP ? (g < 4 ? 0x51u : 0x40u) : 0x51u;
+            const uint32_t s0 = DUP && g >= 4 ? 0x62u : 0x73u;
+            const uint32_t s1 = DUP ? (g < 4 ? 0x51u : 0x40u) : 0x62u;
+            uint32_t low = 0;
 #pragma unroll
             for (int s = 0; s < 8; s++) {
                 uint32_t n[4];
 #pragma unroll
-                for (int u = 0; u < 4; u++)
-                    n[u] = ((uint32_t)__float2int_rn(element(s, u)) + kBias) ^ kBias;
+                for (int u = 0; u < 4; u++) {
+                    const float x = element(s, u);
+                    const int whole = __float2int_rn(x);
+                    left |= (float)whole != x;
+                    n[u] = ((uint32_t)whole + kBias) ^ kBias;
+                }
                 auto digit = [&](uint32_t sel) {
                     return __byte_perm(__byte_perm(n[0], n[1], sel), __byte_perm(n[2], n[3], sel), 0x5410);
                 };
                 f[0][s >> 1][s & 1] = digit(s0);
                 f[1][s >> 1][s & 1] = digit(s1);
-                if constexpr (!DUP)
-                    f[2][s >> 1][s & 1] = digit(0x40u);
+                if constexpr (!DUP) {
+                    f[2][s >> 1][s & 1] = digit(0x51u);
+                    f[3][s >> 1][s & 1] = digit(0x40u);
+                    low |= f[3][s >> 1][s & 1];
+                }
             }
+            deep = !DUP && __any_sync(0xFFFFFFFFu, low != 0u);
         }
+        exact = !__any_sync(0xFFFFFFFFu, left);
         k0 = scale_log2 * __shfl_sync(0xFFFFFFFFu, down, 8 * c);
         k1 = scale_log2 * __shfl_sync(0xFFFFFFFFu, down, 8 * c + 4);
     }
@@ -712,7 +736,7 @@ struct Query {
 #pragma unroll
         for (int i = 0; i < kProducts; i++)
             d[i][0] = d[i][1] = d[i][2] = d[i][3] = 0u;
-        constexpr int kFirst = FMT == RT_KV8_S8 ? kProducts : DUP ? 1 : 2;
+        constexpr int kFirst = kSkips ? kProducts - 1 : kProducts;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const uint4 w = k[j * 32];
@@ -741,9 +765,11 @@ struct Query {
         } else {
 #pragma unroll
             for (int u = 0; u < 4; u++) {
-                const float a = sum_of<FMT>(d[0][u]), b = sum_of<FMT>(d[1][u]), c = sum_of<FMT>(d[2][u]);
-                x[u] = FMT == RT_KV8_E4M3 ? fmaf(fmaf(c, kBase, b), kBase, a)
-                                          : fmaf(fmaf(a, kBase, b), kBase, c);
+                // the larger power of the base first
+                x[u] = sum_of<FMT>(d[FMT == RT_KV8_E4M3 ? kProducts - 1 : 0][u]);
+#pragma unroll
+                for (int i = 1; i < kProducts; i++)
+                    x[u] = fmaf(x[u], kBase, sum_of<FMT>(d[FMT == RT_KV8_E4M3 ? kProducts - 1 - i : i][u]));
             }
         }
     }
@@ -805,6 +831,79 @@ __device__ __forceinline__ void pages_step(Softmax &st, const uint4 *(&blk)[NP],
             if constexpr (!DUP)
                 mma_f16_16816(st.o[2 * j + 1], f, q0, q1);
         }
+    }
+}
+
+// Four codes as two bf16 pairs, exactly.
+template <uint32_t FMT>
+__device__ __forceinline__ void decode4_bf16(uint32_t w, uint32_t &lo, uint32_t &hi)
+{
+    if constexpr (FMT == RT_KV8_E4M3) {
+        decode4<FMT>(w, lo, hi);
+        const float2 a = unpack_f16x2(lo), b = unpack_f16x2(hi);
+        lo = rt::pack_bf16x2(a.x, a.y);
+        hi = rt::pack_bf16x2(b.x, b.y);
+    } else {
+        lo = rt::pack_bf16x2((float)(int8_t)w, (float)(int8_t)(w >> 8));
+        hi = rt::pack_bf16x2((float)(int8_t)(w >> 16), (float)(int8_t)(w >> 24));
+    }
+}
+
+// One page where pages_step's forms do not hold the values: all in bf16, which has the
+// range.  The query as it is, times a power of two, against decoded codes; P in three
+// terms.  With DUP the first four columns carry all of them.  Rare, so it is kept short.
+template <uint32_t FMT, bool DUP>
+__device__ __forceinline__ void wide_step(Softmax &st, const uint4 *blk, const Query<FMT, DUP> &q,
+                                          const __nv_bfloat16 *q_row, bool has_q, float sk, float sv)
+{
+    uint2 qv[8];
+    const int e = Query<FMT, DUP>::exponent(Query<FMT, DUP>::fetch(q_row, has_q, qv));
+    const float up = exp2i(Query<FMT, DUP>::kTop - e);
+    float x[1][4] = {{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const uint4 w = blk[j * 32];
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            const uint2 y = qv[2 * j + s];
+            uint32_t f[4];
+            decode4_bf16<FMT>(s ? w.z : w.x, f[0], f[2]);
+            decode4_bf16<FMT>(s ? w.w : w.y, f[1], f[3]);
+            rt::mma_bf16_16816(x[0], f, rt::pack_bf16x2(bf16_lo(y.x) * up, bf16_hi(y.x) * up),
+                               rt::pack_bf16x2(bf16_lo(y.y) * up, bf16_hi(y.y) * up));
+        }
+    }
+    const float f0 = sk * q.k0, f1 = sk * q.k1;
+    x[0][0] *= f0;
+    x[0][1] *= f1;
+    x[0][2] *= f0;
+    x[0][3] *= f1;
+    softmax_step<1>(st, x);
+    raise_unit(st, unit_of(__float_as_uint(sv) & 0x7FFFFFFFu));
+    const float vf = DUP && (threadIdx.x & 2) ? 0.0f : sv * exp2i(14 - st.v);
+    uint32_t p[3][2];
+#pragma unroll
+    for (int u = 0; u < 4; u++)
+        x[0][u] *= vf;
+#pragma unroll
+    for (int k = 0; k < 3; k++) {
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const uint32_t w = rt::pack_bf16x2(x[0][2 * u], x[0][2 * u + 1]);
+            x[0][2 * u] -= bf16_lo(w);
+            x[0][2 * u + 1] -= bf16_hi(w);
+            p[k][u] = rt::movmatrix_trans(w);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const uint4 w = blk[128 + (i >> 1) * 32];
+        uint32_t f[4];
+        decode4_bf16<FMT>(i & 1 ? w.z : w.x, f[0], f[2]);
+        decode4_bf16<FMT>(i & 1 ? w.w : w.y, f[1], f[3]);
+#pragma unroll
+        for (int k = 0; k < 3; k++)
+            rt::mma_bf16_16816(st.o[i], f, p[k][0], p[k][1]);
     }
 }
 
@@ -1001,7 +1100,14 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) kv8_decode_kernel(con
             const uint8_t *base = slots + s * kEntryBytes;
             const uint4 *blk0 = reinterpret_cast<const uint4 *>(base) + lane;
             const uint4 *blk1 = blk0 + kBlockBytes / 16;
-            if (both == 3u) {
+            if (both != 4u && !q.exact) {
+#pragma unroll 1
+                for (int k = 2 * i; k < 2 * (int)i + 2; k++) {
+                    const float sk = __shfl_sync(0xFFFFFFFFu, sc.x, k), sv = __shfl_sync(0xFFFFFFFFu, sc.y, k);
+                    if (have >> k & 1u)
+                        wide_step<FMT, DUP>(st, k & 1 ? blk1 : blk0, q, q_row, has_q, sk, sv);
+                }
+            } else if (both == 3u) {
                 const uint4 *blk[2] = {blk0, blk1};
                 const float sk[2] = {__shfl_sync(0xFFFFFFFFu, sc.x, 2 * i),
                                      __shfl_sync(0xFFFFFFFFu, sc.x, 2 * i + 1)};

@@ -3,7 +3,7 @@ tolerances are those of test_kv8_gpu.py, except where a test states its own."""
 import pytest
 import torch
 
-from test_kv8_gpu import attend, check, make
+from test_kv8_gpu import KO, attend, check, make
 
 pytestmark = pytest.mark.gpu
 
@@ -55,3 +55,63 @@ def test_attention_of_large_and_small_values(pkg, cuda, fmt, heads, G, pages, ta
     case = (q, codes, scales, rest, table)
     for chunk in (0, 2, 64):
         check(attend(pkg, cuda, *case, long, chunk_pages=chunk), *case, long)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "s8"])
+@pytest.mark.parametrize("heads,G", [(3, 1), (2, 4), (2, 5), (2, 8)])
+@pytest.mark.parametrize("gap", [4, 9, 13, 14, 16, 17, 20, 21, 22, 25, 40, 100])
+def test_attention_of_queries_of_a_wide_range(pkg, cuda, fmt, heads, G, gap):
+    """Elements 2^-gap of their row's largest, where K is 0 at the large ones: the score is the
+    small elements' alone, and as accurate as theirs."""
+    lens = [70, 16, 9, 160, 33]
+    q, pages, scales, tail, table = make(pkg, cuda, lens, heads, G, fmt, seed=54)
+    large = torch.arange(0, 128, 9, device=cuda)
+    at = torch.from_numpy(KO).to(cuda)[:, large].reshape(-1)
+    pages.view(torch.int8)[:, :, 0, at] = 0
+    tail[:, :, 0, :, large] = 0
+    small = torch.ones(128, dtype=torch.bool, device=cuda)
+    small[large] = False
+    q[:, :, large] = torch.where(q[:, :, large] < 0, -1.0, 1.0).bfloat16()
+    q[:, :, small] = (q[:, :, small].float() * 2.0 ** -gap).clamp(-1, 1).bfloat16()
+    q[1] = torch.where(small, 129 / 128 * 2.0 ** -gap, 1.0).bfloat16()
+    q[2, ::2] = q[2, ::2].abs()
+    case = (q, pages, scales, tail, table)
+    scale = 0.08 * 2.0 ** gap
+    check(attend(pkg, cuda, *case, lens, scale=scale), *case, lens, scale)
+    # elements of all sizes in between, and K everywhere
+    q, pages, scales, tail, table = make(pkg, cuda, lens, heads, G, fmt, seed=55)
+    q *= torch.logspace(0, -gap, 128, base=2.0, device=cuda).bfloat16()
+    case = (q, pages, scales, tail, table)
+    check(attend(pkg, cuda, *case, lens, scale=0.3), *case, lens, 0.3)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "s8"])
+@pytest.mark.parametrize("heads,G", [(2, 4), (2, 8)])
+def test_attention_of_a_query_without_numbers(pkg, cuda, fmt, heads, G):
+    """A NaN or an infinity in one head's query is that head's alone, also where its
+    neighbours need all of bf16's range, and a skipped page counts as absent there."""
+    lens = [70, 300]
+    q, pages, scales, tail, table = make(pkg, cuda, lens, heads, G, fmt, seed=56)
+    q[:, :, ::3] *= 2.0 ** -30
+    q[0, 1, 5] = float("nan")
+    q[1, G, 7] = float("inf")
+    case = (q, pages, scales, tail, table)
+    out = attend(pkg, cuda, *case, lens)
+    want = torch.zeros(2, heads * G, dtype=torch.bool, device=cuda)
+    want[0, 1] = want[1, G] = True
+    assert torch.equal(torch.isnan(out).all(-1), want) and torch.equal(torch.isnan(out).any(-1), want)
+    q[0, 1, 5] = q[1, G, 7] = 0
+    clean = attend(pkg, cuda, *case, lens)
+    check(clean, *case, lens)
+    assert torch.equal(out[~want], clean[~want])
+    gone = table.copy()
+    gone[0, 2] = pages.shape[0]
+    error = torch.zeros(1, dtype=torch.int32, device=cuda)
+    got = pkg.kv8_decode_attention(*case[:4], torch.from_numpy(gone).to(cuda),
+                                   torch.tensor(lens, dtype=torch.int32, device=cuda), 300,
+                                   error=error)
+    assert error.item() == 2 and torch.equal(got[1], clean[1])
+    # the same without that page: 54 tokens, the last page one to the left
+    short = table.copy()
+    short[0, 2:-1] = table[0, 3:]
+    check(got[:1], q[:1], pages, scales, tail[:1], short[:1], [54])
