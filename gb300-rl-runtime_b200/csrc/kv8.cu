@@ -502,6 +502,9 @@ struct Softmax {
 
 __device__ __forceinline__ float exp2i(int e) { return __int_as_float((127 + e) << 23); }
 
+// V scales within 2^kFar of the largest leave P 2^-(38 - kFar) of 1 in two fp16 terms.
+constexpr int kFar = 8;
+
 // Bring O to a unit of 2^(v - 14) where it is below.
 __device__ __forceinline__ void raise_unit(Softmax &st, int v)
 {
@@ -575,7 +578,7 @@ __device__ __forceinline__ void softmax_step(Softmax &st, float (&s)[NP][4])
 // hold bf16's 8 bits down to elements 2^-22 (s8), 2^-21 (e4m3, 4 terms) or 2^-17 (3)
 // of the row's largest.  What the last product adds is 0 unless an element is below
 // 2^-14 (s8, more heads) or 2^-13 (e4m3), so most rows skip it (`deep` is false).  Rows
-// with elements that the digits do not hold take wide_step (`exact` is false): K may be
+// with elements that the digits do not hold take wide_step (`left`): K may be
 // 0 where they are large, and then their score is what the small elements say.
 template <uint32_t FMT, bool DUP>
 struct Query {
@@ -586,7 +589,8 @@ struct Query {
     static constexpr int kTop = FMT == RT_KV8_E4M3 ? 7 : 29;
     uint32_t f[kProducts][4][2];
     float k0, k1;  // factors of the scores of the lane's columns 2c and 2c + 1
-    bool deep, exact;  // the same in all lanes
+    bool deep;     // the same in all lanes
+    bool left;     // the digits do not hold the lane's elements
 
     // Row g's elements of the lane, and the bits of the row's largest.
     static __device__ __forceinline__ uint32_t fetch(const __nv_bfloat16 *row, bool has, uint2 (&qv)[8])
@@ -623,7 +627,7 @@ struct Query {
             const uint32_t w = u & 2 ? qv[s].y : qv[s].x;
             return __uint_as_float(u & 1 ? w & 0xFFFF0000u : w << 16) * up;
         };
-        bool left = false;  // something that the digits do not hold
+        left = false;
         if constexpr (FMT == RT_KV8_E4M3) {
             // the first term cut off after 4 bits, the second has the other 4
             bool small = false;
@@ -716,7 +720,6 @@ struct Query {
             }
             deep = !DUP && __any_sync(0xFFFFFFFFu, low != 0u);
         }
-        exact = !__any_sync(0xFFFFFFFFu, left);
         k0 = scale_log2 * __shfl_sync(0xFFFFFFFFu, down, 8 * c);
         k1 = scale_log2 * __shfl_sync(0xFFFFFFFFu, down, 8 * c + 4);
     }
@@ -793,10 +796,6 @@ __device__ __forceinline__ void pages_step(Softmax &st, const uint4 *(&blk)[NP],
         x[p][3] *= f1;
     }
     softmax_step<NP>(st, x);
-    uint32_t top = __float_as_uint(sv[0]) & 0x7FFFFFFFu;
-    if constexpr (NP > 1)
-        top = max(top, __float_as_uint(sv[1]) & 0x7FFFFFFFu);
-    raise_unit(st, unit_of(top));
     const bool low_half = DUP && (threadIdx.x & 2) != 0;  // columns 4..7
 #pragma unroll
     for (int p = 0; p < NP; p++) {
@@ -879,7 +878,6 @@ __device__ __forceinline__ void wide_step(Softmax &st, const uint4 *blk, const Q
     x[0][2] *= f0;
     x[0][3] *= f1;
     softmax_step<1>(st, x);
-    raise_unit(st, unit_of(__float_as_uint(sv) & 0x7FFFFFFFu));
     const float vf = DUP && (threadIdx.x & 2) ? 0.0f : sv * exp2i(14 - st.v);
     uint32_t p[3][2];
 #pragma unroll
@@ -989,9 +987,9 @@ __device__ __forceinline__ void tail_step(Softmax &st, const uint8_t *tk, const 
 // in digits (Query), O^T += V^T.P^T on m16n8k16 with the codes in fp16, exactly;
 // 16 tokens (or 16 dimensions) as rows, the KV group's heads as columns.  K's
 // scale multiplies the scores in fp32.  V's multiplies P: with O's unit 2^(v -
-// 14), v the exponent above the largest scale so far, P times scale fills fp16's
-// range from 2^14 down to 2^-24, and two fp16 terms of it are off by 2^-38 of the
-// largest scale or 2^-22 of their own value.  With up to 4 heads (DUP) columns
+// 14), v the exponent above the largest scale of the warp's pages, P times scale
+// fills fp16's range from 2^14 down to 2^-24, and two fp16 terms of it are off by
+// 2^-38 of the largest scale or 2^-22 of their own value.  With up to 4 heads (DUP) columns
 // 4..7 repeat columns 0..3 and carry P's low terms, so one product covers both (64
 // sequences of up to 4,096, 4 heads, e4m3: 58 us, without 63; s8: 58 and 59).
 template <uint32_t FMT, bool DUP>
@@ -1076,7 +1074,11 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) kv8_decode_kernel(con
     Softmax st;
     st.m0 = st.m1 = -INFINITY;
     st.l0 = st.l1 = 0.0f;
-    st.v = -110;
+    // O's unit holds the warp's largest V scale.  Where another is far below, P would lose
+    // digits of what counts in dimensions that the large ones leave at 0: wide_step.
+    const uint32_t sv_bits = __float_as_uint(sc.y) & 0x7FFFFFFFu;
+    st.v = max(-110, unit_of(__reduce_max_sync(0xFFFFFFFFu, sv_bits)));
+    const bool wide = __any_sync(0xFFFFFFFFu, q.left || (sv_bits != 0u && st.v - unit_of(sv_bits) > kFar));
 #pragma unroll
     for (int i = 0; i < 8; i++)
         st.o[i][0] = st.o[i][1] = st.o[i][2] = st.o[i][3] = 0.0f;
@@ -1100,7 +1102,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) kv8_decode_kernel(con
             const uint8_t *base = slots + s * kEntryBytes;
             const uint4 *blk0 = reinterpret_cast<const uint4 *>(base) + lane;
             const uint4 *blk1 = blk0 + kBlockBytes / 16;
-            if (both != 4u && !q.exact) {
+            if (both != 4u && wide) {
 #pragma unroll 1
                 for (int k = 2 * i; k < 2 * (int)i + 2; k++) {
                     const float sk = __shfl_sync(0xFFFFFFFFu, sc.x, k), sv = __shfl_sync(0xFFFFFFFFu, sc.y, k);

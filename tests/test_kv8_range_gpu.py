@@ -3,7 +3,7 @@ tolerances are those of test_kv8_gpu.py, except where a test states its own."""
 import pytest
 import torch
 
-from test_kv8_gpu import KO, attend, check, make
+from test_kv8_gpu import KO, VO, attend, check, make
 
 pytestmark = pytest.mark.gpu
 
@@ -115,3 +115,33 @@ def test_attention_of_a_query_without_numbers(pkg, cuda, fmt, heads, G):
     short = table.copy()
     short[0, 2:-1] = table[0, 3:]
     check(got[:1], q[:1], pages, scales, tail[:1], short[:1], [54])
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "s8"])
+@pytest.mark.parametrize("heads,G", [(4, 4), (2, 8)])
+@pytest.mark.parametrize("order", ["up", "down", "mixed", "one"])
+@pytest.mark.parametrize("scale", [0.02, 0.5])
+def test_attention_of_value_scales_of_a_wide_range(pkg, cuda, fmt, heads, G, order, scale):
+    """V scales from 2^-40 to 2^40 in one sequence; where the pages of large scales hold zeros
+    the small ones' values are what is left, also beside scores that are far apart."""
+    lens = [16 * 37 + 5, 16 * 8, 31, 16 * 150]
+    q, pages, scales, tail, table = make(pkg, cuda, lens, heads, G, fmt, seed=57)
+    g = torch.Generator(device=cuda).manual_seed(58)
+    some = torch.from_numpy(VO).to(cuda)[:, ::5].reshape(-1)
+    for b, n in enumerate(lens):
+        full = n // 16
+        at = torch.from_numpy(table[b, :full]).to(cuda).long()
+        power = torch.linspace(-40, 40, max(full, 2), device=cuda)[:full].round()
+        if order == "down":
+            power = power.flip(0)
+        elif order == "mixed":
+            power = power[torch.randperm(full, generator=g, device=cuda)]
+        elif order == "one":
+            power = torch.where(torch.arange(full, device=cuda) == full // 2, 40.0, 0.0)
+        scales[at, :, 1] *= (2.0 ** power)[:, None]
+        for page in at[power > power.min() + 6].tolist():
+            pages.view(torch.int8)[page, :, 1, some] = 0
+    tail[:, :, 1, :, ::5] *= 2.0 ** -20
+    case = (q, pages, scales, tail, table)
+    for chunk in (0, 8, 128):
+        check(attend(pkg, cuda, *case, lens, scale=scale, chunk_pages=chunk), *case, lens, scale)
