@@ -587,6 +587,7 @@ struct Query {
     // The row's largest element is brought to [2^kTop, 2^(kTop + 1)): a first digit of up
     // to 63 (s8, with room for the carry) or 256 (e4m3).
     static constexpr int kTop = FMT == RT_KV8_E4M3 ? 7 : 29;
+    static constexpr int kFirstUnit = FMT == RT_KV8_E4M3 ? 0 : 24;  // of the first digit: a score's
     uint32_t f[kProducts][4][2];
     float k0, k1;  // factors of the scores of the lane's columns 2c and 2c + 1
     bool deep;     // the same in all lanes
@@ -622,7 +623,7 @@ struct Query {
         const int e = exponent(top);
         const float up = exp2i(kTop - e);
         // a row with a NaN or an infinity has no digits: its scores become NaN
-        const float down = top >= 0x7F80u ? __int_as_float(0x7FC00000) : exp2i(e - kTop);
+        const float down = top >= 0x7F80u ? __int_as_float(0x7FC00000) : exp2i(e - kTop + kFirstUnit);
         auto element = [&](int s, int u) {
             const uint32_t w = u & 2 ? qv[s].y : qv[s].x;
             return __uint_as_float(u & 1 ? w & 0xFFFF0000u : w << 16) * up;
@@ -753,13 +754,11 @@ struct Query {
                 mma_codes_16832<FMT>(d[kProducts - 1], k[j * 32], f[kProducts - 1][j][0],
                                      f[kProducts - 1][j][1]);
         }
-        constexpr float kBase = FMT == RT_KV8_E4M3 ? 0.0625f : 256.0f;
+        // in units of the first digit, so that k0 and k1 stay in range with the query
+        constexpr float kBase = FMT == RT_KV8_E4M3 ? 0x1p-4f : 0x1p-8f;
         if constexpr (DUP) {
             // digits 0 and 2 in columns 0..3, 1 and 3 in 4..7
-            const bool low = (threadIdx.x & 2) != 0;
-            const float one = FMT == RT_KV8_E4M3 ? (low ? kBase : 1.0f)
-                                                 : (low ? kBase * kBase : kBase * kBase * kBase);
-            const float two = FMT == RT_KV8_E4M3 ? one * kBase * kBase : (low ? 1.0f : kBase);
+            const float one = threadIdx.x & 2 ? kBase : 1.0f, two = one * (kBase * kBase);
 #pragma unroll
             for (int u = 0; u < 4; u++) {
                 x[u] = fmaf(sum_of<FMT>(d[0][u]), one, sum_of<FMT>(d[1][u]) * two);
@@ -768,11 +767,10 @@ struct Query {
         } else {
 #pragma unroll
             for (int u = 0; u < 4; u++) {
-                // the larger power of the base first
-                x[u] = sum_of<FMT>(d[FMT == RT_KV8_E4M3 ? kProducts - 1 : 0][u]);
+                x[u] = sum_of<FMT>(d[kProducts - 1][u]);
 #pragma unroll
-                for (int i = 1; i < kProducts; i++)
-                    x[u] = fmaf(x[u], kBase, sum_of<FMT>(d[FMT == RT_KV8_E4M3 ? kProducts - 1 - i : i][u]));
+                for (int i = kProducts - 2; i >= 0; i--)
+                    x[u] = fmaf(x[u], kBase, sum_of<FMT>(d[i][u]));
             }
         }
     }
@@ -857,7 +855,7 @@ __device__ __forceinline__ void wide_step(Softmax &st, const uint4 *blk, const Q
 {
     uint2 qv[8];
     const int e = Query<FMT, DUP>::exponent(Query<FMT, DUP>::fetch(q_row, has_q, qv));
-    const float up = exp2i(Query<FMT, DUP>::kTop - e);
+    const float up = exp2i(Query<FMT, DUP>::kTop - Query<FMT, DUP>::kFirstUnit - e);
     float x[1][4] = {{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
     for (int j = 0; j < 4; j++) {

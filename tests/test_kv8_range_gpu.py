@@ -145,3 +145,17 @@ def test_attention_of_value_scales_of_a_wide_range(pkg, cuda, fmt, heads, G, ord
     case = (q, pages, scales, tail, table)
     for chunk in (0, 8, 128):
         check(attend(pkg, cuda, *case, lens, scale=scale, chunk_pages=chunk), *case, lens, scale)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "s8"])
+@pytest.mark.parametrize("heads,G", [(2, 4), (2, 8)])
+@pytest.mark.parametrize("power", [-118, -105, -90, 60, 100, 115])
+def test_attention_of_small_queries_and_large_keys(pkg, cuda, fmt, heads, G, power):
+    """Queries around 2^power over keys around 2^-power: ordinary scores."""
+    lens = [70, 16, 9, 300]
+    q, pages, scales, tail, table = make(pkg, cuda, lens, heads, G, fmt, seed=59)
+    q *= 2.0 ** power
+    scales[:, :, 0] *= 2.0 ** -power
+    tail[:, :, 0] *= 2.0 ** -power
+    case = (q, pages, scales, tail, table)
+    check(attend(pkg, cuda, *case, lens), *case, lens)
