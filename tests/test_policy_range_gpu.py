@@ -6,7 +6,9 @@ import math
 import pytest
 import torch
 
-from test_policy_gpu import E, case, grad64, logits_of, policy64, rows64
+import test_policy_gpu
+from test_policy_gpu import (E, case, check_backward, check_forward, check_policy, grad64,
+                             logits_of, policy64, rows64)
 
 pytestmark = pytest.mark.gpu
 
@@ -135,3 +137,26 @@ def test_policy_of_large_divergences(pkg, cuda, dtype, V):
     hit = torch.zeros_like(ref).scatter_(1, tokens.long()[:, None], 1.0)
     tol = tol + (share * slope.abs())[:, None] * (p + hit)
     assert bool(((r.dlogits[ok].double() - ref[ok]).abs() <= tol[ok]).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("R,V", [(600, 6000), (600, 6001), (593, 5999), (592, 6000), (2500, 1000),
+                                 (2500, 1001)])
+@pytest.mark.parametrize("offset,extra", [(0, 0), (3, 5)])
+def test_rows_at_the_edges_of_a_warp(pkg, cuda, monkeypatch, dtype, R, V, offset, extra):
+    """Up to 6,000 logits a row may be a warp's own: each of a lane's two sums has 94 terms, and
+    1 + 6 additions behind them, so with two exponentials' shares the relative error of the sum
+    is at most 1.37 x 2^-22 + 101 x 2^-24 < 6.4e-6."""
+    monkeypatch.setattr(test_policy_gpu, "E", 6.4e-6)
+    logits, tokens = logits_of(cuda, R, V, dtype, V, offset=offset, stride=V + extra)
+    check_forward(pkg, logits, tokens, 0.8)
+    check_backward(pkg, logits, tokens, 0.8)
+    g = torch.linspace(-1, 1, R, device=cuda)
+    want = pkg.token_logprobs_backward(logits, tokens, g, g)
+    flat = torch.empty(R * (V + extra) + offset, dtype=dtype, device=cuda)
+    same = flat[offset:].view(R, V + extra)[:, :V]
+    same.copy_(logits)
+    got = pkg.token_logprobs_backward(same, tokens, g, g, dlogits=same)
+    assert torch.equal(got, want)
+    if not offset:
+        check_policy(pkg, case(cuda, R, V, dtype, R, 20), t=0.8)
