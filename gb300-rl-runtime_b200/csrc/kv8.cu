@@ -10,12 +10,13 @@
 // from call to call, merge included.
 //   append     256 sequences x 1 token, 8 KV heads       5.3 us  (launch and the
 //                                       dependent loads before a row's)
-//              64 prompts of 64..1,024 tokens             46 us  75% of copy
+//              64 prompts of 64..1,024 tokens, bf16       46 us  75% of copy
+//              the same, fp32                             72 us  80%
 //              4 prompts of 30,001..32,768 tokens        127 us  92%
-//   attention  1 sequence of 17 tokens                   4.2 us  (latency)
-//              64 of 128..4,096, 32 heads on 8            58 us  82%
+//   attention  1 sequence of 17 tokens                   4.4 us  (latency)
+//              64 of 128..4,096, 32 heads on 8            60 us  80%
 //              256 of 512..768, 32 heads on 8             63 us  83%
-//              1 of 131,071, 32 heads on 4                28 us  74%
+//              1 of 131,071, 32 heads on 4                29 us  70%
 #include <cuda_fp16.h>
 
 #include <cmath>
@@ -989,7 +990,7 @@ __device__ __forceinline__ void tail_step(Softmax &st, const uint8_t *tk, const 
 // fills fp16's range from 2^14 down to 2^-24, and two fp16 terms of it are off by
 // 2^-38 of the largest scale or 2^-22 of their own value.  With up to 4 heads (DUP) columns
 // 4..7 repeat columns 0..3 and carry P's low terms, so one product covers both (64
-// sequences of up to 4,096, 4 heads, e4m3: 58 us, without 63; s8: 58 and 59).
+// sequences of up to 4,096, 4 heads, e4m3: 59 us, without 64; s8: 59 and 60).
 template <uint32_t FMT, bool DUP>
 __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm) kv8_decode_kernel(const AttnArgs a)
 {
@@ -1290,10 +1291,15 @@ __global__ void __launch_bounds__(WARPS == 1 ? 256 : WARPS * 32) kv8_merge_kerne
 
 // Pages per item.  Where all rows' pages make two items to an SM of up to 128 pages
 // each, so many: fewer leave bandwidth idle, more are merged longer (1 x 131,071
-// tokens, 4 KV heads: 28 us, with 48 pages an item 34, 32: 38).  Larger batches have
+// tokens, 4 KV heads: 29 us, with 48 pages an item 36, 32: 39).  Larger batches have
 // more items than fit at once, and an item's start and end cost about as much as 14
-// pages: 96 pages (64 sequences of up to 4,096: 58 us, with 32 pages 65; 16 of up to
-// 8,192: 34 against 40).
+// pages: 96 pages.  Of nine batches of 16 to 64 sequences of up to 4,096 or 8,192 tokens,
+// 8 KV heads, in both formats, eight are in this class, and 96 is the best of 16, 32,
+// 48, 64, 96 and 128 or within 3% of it (64 of 128..4,096: 59 us, 32 pages 66, 128 62;
+// 16 of 128..8,192: 30, 32 pages 38, 128 32) but for one: 32 of 2,048..4,096, 1.4 turns
+// of the GPU, take 44 and with 128 pages 40, which cost 64 such sequences 80 for 75.
+// 16 of 2,048..4,096 have two items of 128 to an SM: 26 us in s8, 28 in e4m3, 25 and 27
+// with 96.
 struct AttnPlan {
     uint32_t chunk_pages, max_chunks;
     size_t part_o, part_ml;
@@ -1500,7 +1506,7 @@ extern "C" int rt_kv8_decode_attention(const rt_kv8_attn_params_t *p, const void
         // a programmatic dependent: its CTAs are in place when the last items end
         const uint32_t items = p->num_seqs * p->num_q_heads;
         // A warp to a row once rows outweigh chunks: 24 sequences of 8,192 tokens (768 rows,
-        // 6 chunks) 53 us, a CTA each 60; 4 of 32,768 (128 rows, 22 chunks) 56 against 52.
+        // 6 chunks) 76 us, a CTA each 83; 4 of 32,768 (128 rows, 22 chunks) 58 against 52.
         const bool many = items >= 32u * plan.max_chunks;
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(many ? (items + 7u) / 8u : items);

@@ -6,22 +6,23 @@
 // holds a row in shared memory, each of its warps a region that it alone loads
 // (one bulk copy), reduces and turns into gradient, so regions need no barrier of
 // their own; while a row is worked on the next one's copies are under way.  The
-// warps' statistics are exchanged through distributed shared memory, one cluster
-// barrier a row; one warp of each CTA derives the row's coefficients from them,
-// in the same order everywhere.
+// warps send their statistics to every CTA of the cluster, whose mbarrier counts
+// them; one warp of each CTA derives the row's coefficients from them, in the same
+// order everywhere.
 //
 // Exponentials are taken in base 2: with c = log2(e) / T and an integer reference
 // R, e = 2^z, z = l c - R in one fused multiply-add, whose one rounding is that of
-// a small number where e is not small (c's own rounding is a change of T by 2^-25
-// of itself, the same for all elements).  References differ between warps; sums
-// move between them by exact powers of two.
+// a small number where e is not small (c's own three roundings are a change of T by
+// less than 2^-22 of itself, the same for all elements).  References differ between
+// warps; sums move between them by exact powers of two.
 //
 // The floor is the logits read once and the gradient written once, at the rate of a
 // copy (6,547 GB/s measured here).  fp32 is bound by that: 8,192 rows x 32,000 with
 // gradient and entropy 343 us, 93% of copy.  bf16 has two exponentials for every 4
 // bytes that move: 200 us, 80%, with the exponential unit 59% and the issue slots 60%
-// busy (a quarter of the exponentials as polynomials on the multiply-add pipes: 220).  Small calls are bound by latency: 256 rows x 32,000 fp32 without gradient 8.0
-// us (floor 5.0), 64 rows with gradient 8.0 us (floor 2.5).
+// busy (a quarter of the exponentials as polynomials on the multiply-add pipes: 220).
+// Small calls are bound by latency: 256 rows x 32,000 fp32 without gradient 9.4 us
+// (floor 5.0), 64 rows with gradient 8.7 us (floor 2.5).
 #include <cfloat>
 #include <cmath>
 #include <cstdint>
@@ -856,7 +857,7 @@ __global__ void __launch_bounds__(512) policy_stats_kernel(const rt_policy_row_t
 // last (4,096 rows of 8,000 fp32, 6.9 turns: 50 us, one row to a group 62); else one
 // row to a group, balanced by the hardware (1,023 padded rows of 50,001 bf16, 3.5
 // turns: 46 us, shares of 4 51); blocks of 8 where there are many (8,192 rows of
-// 32,000 fp32: 345 us, one row to a group 380).
+// 32,000 fp32: 343 us, one row to a group 380).
 template <typename T, Mode MODE, bool ALONE>
 int launch_rows(RowArgs &a, uint32_t k, cudaStream_t stream, const char *what)
 {

@@ -181,8 +181,8 @@ int rt_attn_plan(const rt_attn_params_t *p, uint32_t *chunk_pages,
  *     scale = max|x| / Q          (Q = 448 for e4m3, 127 for s8; one fp32 division)
  *     code  = round(x / scale)    (fp32 quotient, then to nearest even; |code| <= Q)
  * with scale = 0 and codes 0 for a tile of zeros, and scale = NaN when a tile
- * holds a NaN or an infinity (attention over it is then NaN, as over the
- * values themselves).  Tiles are quantised once, when their 16 tokens are
+ * holds a NaN or an infinity (attention over it is then NaN; over one in a tail
+ * at least where the value has a part).  Tiles are quantised once, when their 16 tokens are
  * there: a sequence of L tokens has L / 16 pages in 8 bits (page_table) and
  * its last L % 16 tokens in bf16, in its entry of `tail`.  So the cache does
  * not depend on how many tokens each call brought, and full pages, which are
@@ -251,6 +251,13 @@ typedef struct {
  * id counts as absent.  `workspace` holds the partial results of sequences that
  * are split (none, 0 bytes, where max_seq_len is short); it needs no
  * initialisation, and calls that share one must not overlap on the GPU.
+ * Accuracy: that of sums in fp32 over bf16 queries and decoded values, whatever
+ * their ranges.  With s = sum |q_d k_d| scale and the weights p, a score is off by
+ * at most 2^-19 s, and the output by 2 (2^-19 max s + 2^-18) sum p |v| and, for each
+ * token, by 2^-38 of the sequence's largest |v|; not held are query elements below
+ * 2^-100 of their head's largest, V scales below 2^-80 of the sequence's largest, and
+ * products of a largest |q| and a largest |k| beyond fp32's range.  Finite V give
+ * finite means.
  * Results do not depend on earlier calls and are the same, bit for bit, in
  * every run of the same shape on the same GPU. */
 size_t rt_kv8_attn_workspace_bytes(const rt_kv8_attn_params_t *p);
