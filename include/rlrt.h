@@ -181,11 +181,11 @@ int rt_attn_plan(const rt_attn_params_t *p, uint32_t *chunk_pages,
  *     scale = max|x| / Q          (Q = 448 for e4m3, 127 for s8; one fp32 division)
  *     code  = round(x / scale)    (fp32 quotient, then to nearest even; |code| <= Q)
  * with scale = 0 and codes 0 for a tile of zeros, and scale = NaN when a tile
- * holds a NaN or an infinity (attention over it is then NaN; over one in a tail
- * at least where the value has a part).  Tiles are quantised once, when their 16 tokens are
- * there: a sequence of L tokens has L / 16 pages in 8 bits (page_table) and
- * its last L % 16 tokens in bf16, in its entry of `tail`.  So the cache does
- * not depend on how many tokens each call brought, and full pages, which are
+ * holds a NaN or an infinity (attention over it is then NaN; over one in a tail's
+ * V, NaN or infinite in that dimension).  Tiles are quantised once, when their 16
+ * tokens are there: a sequence of L tokens has L / 16 pages in 8 bits
+ * (page_table) and its last L % 16 tokens in bf16, in its entry of `tail`.  So the
+ * cache does not depend on how many tokens each call brought, and full pages, which are
  * never written again, can be shared by sequences with a common prefix.
  *
  *   pages  codes, [arena_pages] pages of rt_kv8_page_bytes, order of kv_layout.h

@@ -3,7 +3,7 @@ tolerances are those of test_kv8_gpu.py, except where a test states its own."""
 import pytest
 import torch
 
-from test_kv8_gpu import KO, VO, attend, check, make
+from test_kv8_gpu import KO, VO, attend, check, make, reference
 
 pytestmark = pytest.mark.gpu
 
@@ -159,3 +159,32 @@ def test_attention_of_small_queries_and_large_keys(pkg, cuda, fmt, heads, G, pow
     tail[:, :, 0] *= 2.0 ** -power
     case = (q, pages, scales, tail, table)
     check(attend(pkg, cuda, *case, lens), *case, lens)
+
+
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("heads,G", [(2, 4), (2, 8)])
+def test_attention_of_a_tail_without_numbers(pkg, cuda, heads, G, value):
+    """In V it shows in its head and dimension alone.  In K it makes a score NaN, or infinite:
+    +infinity leaves NaN, -infinity is a weight of 0, the token's absence."""
+    lens = [70, 300]
+    q, pages, scales, tail, table = make(pkg, cuda, lens, heads, G, "s8", seed=60)
+    clean = attend(pkg, cuda, q, pages, scales, tail, table, lens)
+    v = tail.clone()
+    v[0, 0, 1, 3, 7] = value
+    out = attend(pkg, cuda, q, pages, scales, v, table, lens)
+    hit = torch.zeros_like(out, dtype=torch.bool)
+    hit[0, :G, 7] = True
+    assert torch.equal(~torch.isfinite(out), hit) and torch.equal(out[~hit], clean[~hit])
+    k = tail.clone()
+    k[0, 0, 0, 3, 7] = value
+    out = attend(pkg, cuda, q, pages, scales, k, table, lens)
+    sign = value * q[0, :G, 7].float()
+    nan = torch.zeros_like(hit)
+    nan[0, :G] = ~(sign < 0)[:, None]
+    assert torch.equal(torch.isnan(out), nan)
+    assert torch.equal(out[0, G:], clean[0, G:]) and torch.equal(out[1], clean[1])
+    short = tail.clone()
+    short[0, :, :, 3:5] = tail[0, :, :, 4:6]
+    ref, bound = reference(q, pages, scales, short, table, [69, 300], 0, 128 ** -0.5)
+    near = (out[0, :G].double() - ref[:G]).abs() <= bound[:G]
+    assert bool((near | nan[0, :G]).all())
